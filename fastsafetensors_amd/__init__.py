@@ -11,6 +11,7 @@ from .frameworks._torch import StubProcessGroup
 from .loader import BaseSafeTensorsFileLoader, SafeTensorsFileLoader, fastsafe_open
 from .parallel_loader import ParallelLoader, PipelineParallel
 from .st_types import Device, DeviceType, DType
+from .updates import LowRankUpdate, merge_low_rank
 
 __all__ = [
     "BaseSafeTensorsFileLoader",
@@ -18,6 +19,7 @@ __all__ = [
     "DeviceType",
     "DType",
     "FilesBufferOnDevice",
+    "LowRankUpdate",
     "ParallelLoader",
     "PipelineParallel",
     "SafeTensorsFileLoader",
@@ -28,5 +30,6 @@ __all__ = [
     "fastsafe_open",
     "get_device_numa_node",
     "hold_reader",
+    "merge_low_rank",
     "release_cached_memory",
 ]

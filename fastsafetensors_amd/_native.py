@@ -145,6 +145,31 @@ class FstxConvertDesc(ctypes.Structure):
     ]
 
 
+class FstxLowRankDesc(ctypes.Structure):
+    _fields_ = [
+        ("dst", ctypes.c_void_p),
+        ("src", ctypes.c_void_p),
+        ("up", ctypes.c_void_p),
+        ("down", ctypes.c_void_p),
+        ("weight_scale", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("cols", ctypes.c_uint64),
+        ("rank", ctypes.c_uint64),
+        ("dst_pitch", ctypes.c_uint64),
+        ("src_pitch", ctypes.c_uint64),
+        ("up_row_stride", ctypes.c_uint64),
+        ("up_col_stride", ctypes.c_uint64),
+        ("down_row_stride", ctypes.c_uint64),
+        ("down_col_stride", ctypes.c_uint64),
+        ("scale", ctypes.c_float),
+        ("type", ctypes.c_uint32),
+        ("up_type", ctypes.c_uint32),
+        ("down_type", ctypes.c_uint32),
+        ("n_weight_scales", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
 ELEM_TYPES = {"F64": 0, "F32": 1, "F16": 2, "BF16": 3, "F8_E4M3": 4, "F8_E5M2": 5}
 _ELEM_BYTES = {"F64": 8, "F32": 4, "F16": 2, "BF16": 2, "F8_E4M3": 1, "F8_E5M2": 1}
 
@@ -210,6 +235,15 @@ _SIGNATURES = {
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
+# the same for include/fstx_update.h (kernels that change loaded weights)
+_UPDATE_SIGNATURES = {
+    "fstx_merge_low_rank_workspace": (ctypes.c_int64, [ctypes.POINTER(FstxLowRankDesc), ctypes.c_uint32]),
+    "fstx_merge_low_rank": (
+        ctypes.c_int, [ctypes.POINTER(FstxLowRankDesc), ctypes.c_uint32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
+}
+
+UPDATE_SYMBOLS = tuple(_UPDATE_SIGNATURES)
+
 
 def library_path() -> str:
     """``libfstx.so`` next to this file, or the build named by ``FSTX_LIBRARY``."""
@@ -230,7 +264,7 @@ def lib() -> ctypes.CDLL:
                     "(needs hipcc); this package has no fallback without its HIP library"
                 )
             handle = ctypes.CDLL(path)
-            for name, (restype, argtypes) in _SIGNATURES.items():
+            for name, (restype, argtypes) in (*_SIGNATURES.items(), *_UPDATE_SIGNATURES.items()):
                 fn = getattr(handle, name)
                 fn.restype = restype
                 fn.argtypes = argtypes
@@ -449,6 +483,15 @@ def convert_batch(jobs: Sequence[Tuple[int, int, int, int, int]], stream: int = 
         part = jobs[i : i + FSTX_BATCH_MAX]
         arr = (FstxConvertDesc * len(part))(*[FstxConvertDesc(*j) for j in part])
         _check("fstx_convert_batch", lib().fstx_convert_batch(arr, len(part), stream))
+
+
+def merge_low_rank_workspace(descs: Any, n: int) -> int:
+    """Workspace bytes of ``n`` descriptors (a ctypes array); all of their arguments are checked."""
+    return _check("fstx_merge_low_rank", lib().fstx_merge_low_rank_workspace(descs, n))
+
+
+def merge_low_rank(descs: Any, n: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    _check("fstx_merge_low_rank", lib().fstx_merge_low_rank(descs, n, workspace, workspace_bytes, stream))
 
 
 # ---- reader ------------------------------------------------------------------------------

@@ -44,6 +44,8 @@ int check_launch(const char *what);  // hipGetLastError -> 0 / -FSTX_E_HIP
 // 1 (default) it serves every strided shape but dense cuts that are 16-byte aligned throughout,
 // 2 those too
 int gather_mode();
+// dies the current device deals workgroups out to, as log2 (see tile_for_die in fstx_gather_core.h)
+uint32_t dies_log2();
 bool debug_enabled();
 void debug(const char *fmt, ...) __attribute__((format(printf, 1, 2)));
 void note_bounce_bytes(int64_t delta); // process-wide pinned ring accounting

@@ -860,6 +860,8 @@ struct GatherBatch {
 
 } // namespace
 
+uint32_t fstx_internal::dies_log2() { return ::dies_log2(); }
+
 extern "C" int fstx_realign_copy_batch(const fstx_copy_desc *descs, uint32_t n, void *stream) {
     if (n == 0) return 0;
     if (!descs) return -FSTX_E_INVAL;

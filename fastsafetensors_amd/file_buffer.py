@@ -13,6 +13,7 @@ of a file are cut by ONE batched kernel launch instead of one strided copy per
 tensor.
 """
 
+import re
 from collections import OrderedDict
 from typing import Any, Dict, List, Optional, Tuple
 
@@ -22,6 +23,9 @@ from .st_types import Device, DType
 from .tensor_factory import LazyTensorFactory
 
 logger = init_logger(__name__)
+
+# "<module>.lora_A.weight", or with the adapter's name in between ("<module>.lora_A.default.weight")
+_ADAPTER_KEY = re.compile(r"(?P<module>.+)\.lora_(?P<which>[AB])(\.[^.]+)?\.weight$")
 
 
 class FilesBufferOnDevice:
@@ -198,3 +202,59 @@ class FilesBufferOnDevice:
             run.append((name, dim))
         flush()
         return {name: out[name] for name in tensor_shard_dim}
+
+    # -- changing the loaded weights ----------------------------------------------------
+    def merge_adapter(
+        self,
+        adapter: "FilesBufferOnDevice",
+        alpha: Optional[float] = None,
+        scale: Optional[float] = None,
+        prefix: str = "base_model.model.",
+        fan_in_fan_out: bool = False,
+    ) -> List[str]:
+        """Merge the low-rank adapter loaded as ``adapter`` into the weights of this object, in place:
+        ``W += s * (lora_B @ lora_A)`` for every pair ``<prefix><module>.lora_A.weight`` /
+        ``.lora_B.weight``, ``W`` being ``<module>.weight``.  Returns the names of the weights.
+
+        ``s`` is ``scale``, or ``alpha / rank`` of each pair (one of the two has to be given).
+        ``fan_in_fan_out``: the weights are stored ``[in, out]`` (GPT-2).  fp8 e4m3 weights are taken
+        with their ``<module>.weight_scale`` and requantised to it.  A negative ``scale`` takes an
+        adapter out again, up to the rounding of the weights' type.
+
+        Everything is checked before the first weight changes: a tensor of the adapter that is
+        neither of a pair's, a pair without its weight, or shapes that do not match raise.  All
+        merges leave as a handful of launches on the current stream.  Whatever was cut or
+        joined from these weights before keeps their old values; views of them show the new ones."""
+        if (alpha is None) == (scale is None):
+            raise ValueError("merge_adapter: give either alpha or scale")
+        pairs: Dict[str, Dict[str, str]] = {}
+        for key in adapter.key_to_rank_lidx:
+            m = _ADAPTER_KEY.match(key)
+            if m is None:
+                raise ValueError(f"merge_adapter: {key} is not a lora_A / lora_B weight")
+            module = m.group("module")
+            module = module[len(prefix) :] if prefix and module.startswith(prefix) else module
+            if pairs.setdefault(module, {}).setdefault(m.group("which"), key) != key:
+                raise ValueError(f"merge_adapter: more than one lora_{m.group('which')} for {module}")
+        items, names, factories = [], [], []
+        for module, pair in pairs.items():
+            name = f"{module}.weight"
+            if len(pair) != 2:
+                raise ValueError(f"merge_adapter: {module} has only one of lora_A and lora_B")
+            if name not in self.key_to_rank_lidx:
+                raise ValueError(f"merge_adapter: {name} was not found in files")
+            factory = self._factory(name)[2]
+            weight = factory._held(name, "merge_adapter")
+            a, b = (adapter._factory(pair[k])[2]._held(pair[k], "merge_adapter") for k in "AB")
+            weight_scale = None
+            if weight.dtype == DType.F8_E4M3:
+                if f"{name}_scale" not in self.key_to_rank_lidx:
+                    raise ValueError(f"merge_adapter: {name} is fp8 and {name}_scale was not found in files")
+                weight_scale = self._factory(f"{name}_scale")[2]._held(f"{name}_scale", "merge_adapter")
+            items.append((weight, a, b, weight_scale))
+            names.append(name)
+            factories.append(factory)
+        self.framework.merge_adapters(items, alpha, scale, fan_in_fan_out)
+        for name, factory in zip(names, factories):
+            factory.shuffled.pop(name, None)  # a shard kept from before the merge is not this weight's any more
+        return names

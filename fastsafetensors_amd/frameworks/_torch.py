@@ -27,6 +27,7 @@ import torch
 from .. import _native
 from ..common import SingleGroup, TensorFrame
 from ..st_types import Device, DeviceType, DType, dtype_size
+from ..updates import LowRankUpdate, merge_low_rank
 from . import FrameworkOpBase, ProcessGroupBase, TensorBase
 
 dtype_convert: Dict[DType, torch.dtype] = {
@@ -506,6 +507,25 @@ class TorchOp(FrameworkOpBase):
             strides = tuple(math.prod(shape[d + 1 :]) for d in range(len(shape)))
             outs.append(TorchTensor(src0.device, src0.dtype, torch.as_strided(flats[tdt], shape, strides, at)))
         return outs
+
+    # ---- changing loaded weights -----------------------------------------------
+    def merge_adapters(
+        self,
+        items: List[Tuple[TorchTensor, TorchTensor, TorchTensor, Optional[TorchTensor]]],
+        alpha: Optional[float],
+        scale: Optional[float],
+        fan_in_fan_out: bool,
+    ) -> None:
+        updates = []
+        for weight, a, b, weight_scale in items:
+            lora_a, lora_b = a.real_tensor, b.real_tensor
+            if lora_a.dim() != 2 or lora_b.dim() != 2:
+                raise ValueError(f"adapter factors must have two dimensions, not {tuple(lora_a.shape)} and {tuple(lora_b.shape)}")
+            s = scale if scale is not None else alpha / max(lora_a.shape[0], 1)
+            up, down = (lora_a.t(), lora_b.t()) if fan_in_fan_out else (lora_b, lora_a)
+            updates.append(LowRankUpdate(weight.real_tensor, up, down, s,
+                                         None if weight_scale is None else weight_scale.real_tensor))
+        merge_low_rank(updates)
 
     # ---- misc ------------------------------------------------------------------
     def synchronize(self, device: Device) -> None:
