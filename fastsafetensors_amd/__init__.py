@@ -11,7 +11,7 @@ from .frameworks._torch import StubProcessGroup
 from .loader import BaseSafeTensorsFileLoader, SafeTensorsFileLoader, fastsafe_open
 from .parallel_loader import ParallelLoader, PipelineParallel
 from .st_types import Device, DeviceType, DType
-from .updates import LowRankUpdate, merge_low_rank
+from .updates import LowRankUpdate, merge_low_rank, orthogonalize
 
 __all__ = [
     "BaseSafeTensorsFileLoader",
@@ -31,5 +31,6 @@ __all__ = [
     "get_device_numa_node",
     "hold_reader",
     "merge_low_rank",
+    "orthogonalize",
     "release_cached_memory",
 ]

@@ -170,6 +170,20 @@ class FstxLowRankDesc(ctypes.Structure):
     ]
 
 
+class FstxOrthogonalizeDesc(ctypes.Structure):
+    _fields_ = [
+        ("dst", ctypes.c_void_p),
+        ("src", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("cols", ctypes.c_uint64),
+        ("dst_pitch", ctypes.c_uint64),
+        ("src_row_stride", ctypes.c_uint64),
+        ("src_col_stride", ctypes.c_uint64),
+        ("type", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
 ELEM_TYPES = {"F64": 0, "F32": 1, "F16": 2, "BF16": 3, "F8_E4M3": 4, "F8_E5M2": 5}
 _ELEM_BYTES = {"F64": 8, "F32": 4, "F16": 2, "BF16": 2, "F8_E4M3": 1, "F8_E5M2": 1}
 
@@ -240,6 +254,10 @@ _UPDATE_SIGNATURES = {
     "fstx_merge_low_rank_workspace": (ctypes.c_int64, [ctypes.POINTER(FstxLowRankDesc), ctypes.c_uint32]),
     "fstx_merge_low_rank": (
         ctypes.c_int, [ctypes.POINTER(FstxLowRankDesc), ctypes.c_uint32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
+    "fstx_orthogonalize_workspace": (ctypes.c_int64, [ctypes.POINTER(FstxOrthogonalizeDesc), ctypes.c_uint32]),
+    "fstx_orthogonalize": (
+        ctypes.c_int, [ctypes.POINTER(FstxOrthogonalizeDesc), ctypes.c_uint32, ctypes.POINTER(ctypes.c_float), ctypes.c_uint32,
+                       ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
 }
 
 UPDATE_SYMBOLS = tuple(_UPDATE_SIGNATURES)
@@ -492,6 +510,17 @@ def merge_low_rank_workspace(descs: Any, n: int) -> int:
 
 def merge_low_rank(descs: Any, n: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
     _check("fstx_merge_low_rank", lib().fstx_merge_low_rank(descs, n, workspace, workspace_bytes, stream))
+
+
+def orthogonalize_workspace(descs: Any, n: int) -> int:
+    """Workspace bytes of ``n`` descriptors (a ctypes array); all of their arguments are checked."""
+    return _check("fstx_orthogonalize", lib().fstx_orthogonalize_workspace(descs, n))
+
+
+def orthogonalize(descs: Any, n: int, coefficients: Any, steps: int, eps: float, workspace: int, workspace_bytes: int,
+                  stream: int = 0) -> None:
+    _check("fstx_orthogonalize",
+           lib().fstx_orthogonalize(descs, n, coefficients, steps, eps, workspace, workspace_bytes, stream))
 
 
 # ---- reader ------------------------------------------------------------------------------

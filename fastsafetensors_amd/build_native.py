@@ -16,7 +16,7 @@ from typing import List
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = ["fstx_kernels.hip", "fstx_low_rank.hip", "fstx_device_hip.cpp", "fstx_pipeline.cpp"]
+SOURCES = ["fstx_kernels.hip", "fstx_low_rank.hip", "fstx_orthogonalize.hip", "fstx_device_hip.cpp", "fstx_pipeline.cpp"]
 OUTPUT = os.path.join(HERE, "libfstx.so")
 
 

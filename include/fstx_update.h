@@ -51,6 +51,30 @@ int64_t fstx_merge_low_rank_workspace(const fstx_low_rank_desc *descs, uint32_t 
 int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, void *workspace,
                         uint64_t workspace_bytes, void *stream);
 
+/* dst = the nearest orthogonal matrix of src, approximated by `steps` Newton-Schulz steps:
+ *   X = src / (|src|_F + eps);   per step (a, b, c):  A = X X^T,  X <- a X + (b A + c A A) X
+ * with the shorter side as rows (orthogonal rows if rows <= cols, else orthogonal columns).  Products
+ * are as accurate as 32-bit ones; sums are held in 32 bits, the norm in 64.  While the steps run the
+ * iterates' singular values have to stay below about 2 (those of X start at 1 or less). */
+typedef struct fstx_orthogonalize_desc {
+    void *dst;                              /* [rows, cols] of `type`, rows dst_pitch elements apart     */
+    const void *src;                        /* [rows, cols] of `type`, any strides (elements); may be dst */
+    uint64_t rows, cols;                    /* up to 2^20, the smaller one up to 2^16                    */
+    uint64_t dst_pitch;
+    uint64_t src_row_stride, src_col_stride;
+    uint32_t type;                          /* FSTX_F32, FSTX_F16 or FSTX_BF16                           */
+    uint32_t reserved;
+} fstx_orthogonalize_desc;
+
+/* Bytes of workspace for these descriptors, or a negative status. */
+int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *descs, uint32_t n);
+
+/* Any number of matrices; those that fit one set of launches together run together.  `coefficients`
+ * (host memory) are a, b, c of each of the 1..64 steps.  No destination may overlap another
+ * descriptor's source or destination. */
+int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t n, const float *coefficients, uint32_t steps,
+                       float eps, void *workspace, uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
