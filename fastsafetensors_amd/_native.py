@@ -254,7 +254,8 @@ _UPDATE_SIGNATURES = {
     "fstx_merge_low_rank_workspace": (ctypes.c_int64, [ctypes.POINTER(FstxLowRankDesc), ctypes.c_uint32]),
     "fstx_merge_low_rank": (
         ctypes.c_int, [ctypes.POINTER(FstxLowRankDesc), ctypes.c_uint32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
-    "fstx_orthogonalize_workspace": (ctypes.c_int64, [ctypes.POINTER(FstxOrthogonalizeDesc), ctypes.c_uint32]),
+    "fstx_orthogonalize_workspace": (
+        ctypes.c_int64, [ctypes.POINTER(FstxOrthogonalizeDesc), ctypes.c_uint32, ctypes.POINTER(ctypes.c_float), ctypes.c_uint32]),
     "fstx_orthogonalize": (
         ctypes.c_int, [ctypes.POINTER(FstxOrthogonalizeDesc), ctypes.c_uint32, ctypes.POINTER(ctypes.c_float), ctypes.c_uint32,
                        ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
@@ -512,9 +513,9 @@ def merge_low_rank(descs: Any, n: int, workspace: int, workspace_bytes: int, str
     _check("fstx_merge_low_rank", lib().fstx_merge_low_rank(descs, n, workspace, workspace_bytes, stream))
 
 
-def orthogonalize_workspace(descs: Any, n: int) -> int:
+def orthogonalize_workspace(descs: Any, n: int, coefficients: Any, steps: int) -> int:
     """Workspace bytes of ``n`` descriptors (a ctypes array); all of their arguments are checked."""
-    return _check("fstx_orthogonalize", lib().fstx_orthogonalize_workspace(descs, n))
+    return _check("fstx_orthogonalize", lib().fstx_orthogonalize_workspace(descs, n, coefficients, steps))
 
 
 def orthogonalize(descs: Any, n: int, coefficients: Any, steps: int, eps: float, workspace: int, workspace_bytes: int,

@@ -17,19 +17,19 @@
 // the ten times of fp32 MFMA.  One term is not enough: the iteration multiplies small singular values by a
 // each step, and with them the rounding errors of the first steps, up to a^steps = 485 times;
 // with a few strong directions over a floor of weak ones a single fp16 term ends 2 to 3 % off (bf16:
-// 20 %), measured on spectra with a ratio of 1000.  Errors of the LAST step are not amplified any more: where
-// the result is rounded to bf16 (2^-9) it runs on one term, which costs 2^-11 or so.
+// 20 %), measured on spectra with a ratio of 1000.  What has to keep both terms is X itself, in a X; whether the
+// products of a step need them depends on how large B X is beside a X, see one_term_steps.
 // fp16 rather than bf16 terms because the iterates are bounded: entries of X are at most about
 // 1.2, they are held times a power of two near sqrt(p q) so that their typical size stays in the
 // middle of fp16's range; A and B are held times fixed powers of two likewise.
 //
 // Operand layout.  A matrix [R, K] that enters a product as rows x K is stored as blocks of 32
 // rows x 16 k in the lane order of v_mfma_f32_32x32x16 (lane: row lane % 32, k = 8 (lane / 32) + 0..7), 1 KiB
-// per block and term, terms adjacent, blocks of one row of blocks adjacent.  Tiles then go
+// per block, blocks of one row of blocks adjacent, the second term a whole matrix behind the first.  Tiles go
 // from memory to LDS with global_load_lds as they are, and from LDS to registers as
 // conflict-free 16-byte reads.  Products run transposed (the second operand first), so that a
 // lane holds four consecutive k of one row of the result seen as an operand: results go back to that
-// layout in 8-byte stores.  The transposed copy that the next product needs (X^T; the tile mirrored
+// layout in 8-byte stores, 512 contiguous bytes per instruction.  The transposed copy that the next product needs (X^T; the tile mirrored
 // at the diagonal) is made in registers by an MFMA with the identity, which is exact.
 // Sides are padded with zeros to whole tiles; products of zeros stay zeros, nothing is masked.
 
@@ -46,23 +46,24 @@ namespace {
 #define FSTX_GLOBAL __attribute__((address_space(1)))
 #define FSTX_LDS __attribute__((address_space(3)))
 typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 half_t;
 
 constexpr uint32_t kBlk = 512;        // elements of one block (32 rows x 16 k) of one term
-constexpr uint32_t kPad = 256;        // sides are stored padded to this
-constexpr uint32_t kStepPad = 64;     // ... and computed padded to this
+constexpr uint32_t kPadP = 256, kPadQ = 256; // sides are stored padded to these (the largest tile)
+constexpr uint32_t kStepPad = 64;            // ... and summed over padded to this
 constexpr uint32_t kMaxJobs = 20;
-constexpr uint32_t kPartials = 256;   // partial sums of squares per matrix
+constexpr uint32_t kPartials = 1024;         // partial sums of squares per matrix
 constexpr float kScaleA = 2048.0f;    // A is held times this
 
-struct Job {
+struct alignas(64) Job {
     const char *src;
     char *dst;
     half_t *x;        // [p, q]
-    half_t *xt[2];    // [q, p], the current one and the next
+    half_t *xt0, *xt1; // [q, p], the current one and the next in turn
     half_t *a, *b;    // [p, p]
     double *partials;
     uint64_t x_row, x_col;   // strides of G seen as X, elements
@@ -77,8 +78,32 @@ static_assert(sizeof(Job) == 128, "20 of them fit the kernel arguments");
 
 struct Jobs {
     Job job[kMaxJobs];
-    uint32_t first[kMaxJobs];
+    uint32_t first[kMaxJobs]; // first workgroup of each job; unused entries ~0
 };
+
+// How one product's tiles are dealt to workgroups (see Launcher::deal): the first `whole` tiles of a job
+// take one workgroup each, the others `split` each, which leave partial sums.
+struct Deal {
+    uint32_t whole[kMaxJobs];
+    uint32_t slot[kMaxJobs];   // where the job's partial sums begin, in tiles
+    float *sums;
+    uint32_t split, dies_log2;
+};
+
+// (by value: a conditional between two members is a conditional between their addresses)
+template <typename T> __device__ __forceinline__ T pick(bool first, T a, T b) { return first ? a : b; }
+
+// The whole job in two wide scalar loads: a copy, because conditional reads through a reference into the
+// kernel's arguments end up as a copy of all of them in scratch memory.
+__device__ __forceinline__ Job fetch_job(const Jobs &t, uint32_t ji) {
+    typedef uint32_t v16u __attribute__((ext_vector_type(16)));
+    const v16u *raw = reinterpret_cast<const v16u *>(&t.job[ji]);
+    const v16u lo = raw[0], hi = raw[1];
+    Job out;
+    __builtin_memcpy(&out, &lo, 64);
+    __builtin_memcpy(reinterpret_cast<char *>(&out) + 64, &hi, 64);
+    return out;
+}
 
 __device__ __forceinline__ uint32_t job_of(const Jobs &t, uint32_t b) {
     uint32_t ji = 0;
@@ -96,6 +121,39 @@ __device__ __forceinline__ float load_elem(const char *src, uint64_t at, uint32_
     return (float)__builtin_bit_cast(half_t, raw);
 }
 
+// N consecutive elements, 16 bytes per load, as aligned as one element
+template <uint32_t N> __device__ __forceinline__ void load_run(const char *src, uint64_t at, uint32_t type, float (&v)[N]) {
+    typedef v4u by2 __attribute__((aligned(2)));
+    typedef v4u by4 __attribute__((aligned(4)));
+    if (type == FSTX_F32) {
+#pragma unroll
+        for (uint32_t k = 0; k < N; k += 4) {
+            const v4u raw = *(const FSTX_GLOBAL by4 *)(src + (at + k) * 4);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const uint32_t bits = raw[e];
+                v[k + e] = __builtin_bit_cast(float, bits);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < N; k += 8) {
+        const v4u raw = *(const FSTX_GLOBAL by2 *)(src + (at + k) * 2);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            const uint32_t lo = raw[e] << 16, hi = raw[e] & 0xffff0000u;
+            if (type == FSTX_BF16) {
+                v[k + 2 * e] = __builtin_bit_cast(float, lo);
+                v[k + 2 * e + 1] = __builtin_bit_cast(float, hi);
+            } else {
+                v[k + 2 * e] = (float)__builtin_bit_cast(half_t, (uint16_t)(lo >> 16));
+                v[k + 2 * e + 1] = (float)__builtin_bit_cast(half_t, (uint16_t)(hi >> 16));
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------ |G|_F and the first operands
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -104,68 +162,80 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
+// G seen with the side along which memory runs as columns, whichever of X's sides that is
+struct View {
+    uint64_t row_stride, col_stride;
+    uint32_t rows, cols;
+    bool x_cols; // the columns are X's columns
+};
+__device__ __forceinline__ View view_of(const Job &job) {
+    if (job.x_col <= job.x_row) return View{job.x_row, job.x_col, job.p, job.q, true};
+    return View{job.x_col, job.x_row, job.q, job.p, false};
+}
+
 // Partial sums of squares in 64 bits, each workgroup its own rows in a fixed order: the sum does
 // not depend on which workgroup ends first, and squares of the largest floats do not overflow.
 __global__ __launch_bounds__(256) void sum_squares_kernel(const Jobs t) {
     __shared__ double part[4];
     const uint32_t ji = job_of(t, blockIdx.x);
-    const Job &job = t.job[ji];
+    const Job job = fetch_job(t, ji);
+    const View g = view_of(job);
     const uint32_t me = blockIdx.x - t.first[ji];
+    // the matrix as one run of pieces of up to 2048 elements of a row, dealt out in turn
+    const uint32_t pieces = (g.cols + 2047) / 2048;
     uint32_t across = 256; // threads along a row
-    while (across > 1 && across / 2 >= job.q) across /= 2;
-    const uint32_t down = 256 / across;
+    while (across > 1 && across / 2 >= g.cols) across /= 2;
+    const uint32_t down = 256 / across, in_row = threadIdx.x % across;
     double sum = 0;
-    for (uint64_t i = (uint64_t)me * down + threadIdx.x / across; i < job.p; i += (uint64_t)job.n_partials * down)
-        for (uint32_t j = threadIdx.x % across; j < job.q; j += across) {
-            const double v = load_elem(job.src, i * job.x_row + (uint64_t)j * job.x_col, job.type);
-            sum += v * v;
+    for (uint64_t i = me; i * down < (uint64_t)g.rows * pieces; i += job.n_partials) {
+        const uint64_t piece = i * down + threadIdx.x / across; // (more than one row at a time only where pieces == 1)
+        const uint64_t row = piece / pieces;
+        if (row >= g.rows) continue;
+        const uint32_t first = (uint32_t)(piece - row * pieces) * 2048;
+        float v[8];
+        if (g.col_stride == 1 && first + 2048 <= g.cols) { // eight consecutive elements per thread
+            load_run<8>(job.src, row * g.row_stride + first + threadIdx.x * 8, job.type, v);
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint32_t c = first + in_row + k * across;
+                v[k] = c < g.cols && (k == 0 || across == 256) ? load_elem(job.src, row * g.row_stride + (uint64_t)c * g.col_stride, job.type) : 0.0f;
+            }
         }
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) sum += (double)v[k] * (double)v[k];
+    }
     sum = wave_sum(sum);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = sum;
     __syncthreads();
     if (threadIdx.x == 0) job.partials[me] = part[0] + part[1] + part[2] + part[3];
 }
 
-// Four wavefronts, one operand block of X or of X^T each.
-__global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const float eps) {
-    const uint32_t ji = job_of(t, blockIdx.x);
-    const Job &job = t.job[ji];
-    double sum = 0;
-    for (uint32_t i = threadIdx.x & 63; i < job.n_partials; i += 64) sum += job.partials[i];
-    const float norm = (float)sqrt(wave_sum(sum));
-    const float factor = job.scale / (norm + eps);
-
-    const uint32_t pp = pad_to(job.p, kPad), qp = pad_to(job.q, kPad);
-    const uint32_t per_side = (pp / 32) * (qp / 16); // the same for both orders
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t blk = (blockIdx.x - t.first[ji]) * 4 + threadIdx.x / 64;
-    const bool second = blk >= per_side;
-    if (second) blk -= per_side;
-    if (blk >= per_side) return;
-    const uint32_t rows = second ? job.q : job.p, ks = second ? job.p : job.q;
-    const uint64_t row_stride = second ? job.x_col : job.x_row, k_stride = second ? job.x_row : job.x_col;
-    const uint32_t k_blocks = (second ? pp : qp) / 16;
-    const uint32_t rb = blk / k_blocks, kb = blk - rb * k_blocks;
-    const uint32_t row = rb * 32 + (lane & 31), k0 = kb * 16 + 8 * (lane >> 5);
-    v8h h, l;
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) {
-        const float v = row < rows && k0 + e < ks
-                            ? load_elem(job.src, (uint64_t)row * row_stride + (uint64_t)(k0 + e) * k_stride, job.type) * factor : 0.0f;
-        h[e] = (half_t)v;
-        l[e] = (half_t)(v - (float)h[e]);
-    }
-    half_t *out = (second ? job.xt[0] : job.x) + (uint64_t)blk * 2 * kBlk + lane * 8;
-    *(FSTX_GLOBAL v8h *)out = h;
-    *(FSTX_GLOBAL v8h *)(out + kBlk) = l;
-}
-
 // ------------------------------------------------------------ the products
 
-// C = P Q^T over whole tiles: TR x TC per workgroup of four wavefronts (2 x 2), k in stages of which one is
-// computed on while the next two are on their way to LDS.  Measured on a [14336, 4096] update, the product of
-// 2 x 4096^2 x 14336 operations in two terms: 128 x 128 tiles 1.45 ms with stages of 32 k and one stage ahead, 1.2 to 1.3 with
-// stages of 16 k and two ahead, 256 x 128 tiles 1.15 ms (1.25 PFLOP/s of fp16 products; fewer LDS reads per product).
+// Waits until at most `left` of this wavefront's global loads are on their way and none of its LDS
+// reads, then for the other wavefronts.  (The empty statements keep the compiler from moving memory accesses
+// across; the wait is the builtin, which it takes into account when it places its own.)
+template <uint32_t left> __device__ __forceinline__ void wait_and_meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (left & 15) | (left >> 4) << 14);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// C = P Q^T over whole tiles: TR x TC per workgroup of four wavefronts (2 x 2), k in stages.  While one stage is
+// multiplied from registers the next one is read from LDS into other registers and two more are on
+// their way from memory to LDS; reads and loads are issued in between the products.
+//
+// What bounds it.  B X of a [14336, 4096] update, 0.48 * 10^15 operations in fp16: two terms (three products) 1.07 to
+// 1.2 ms with 256 x 256 tiles, 1.2 to 1.35 PFLOP/s; the library's 8192^3 fp16 product does 1.3 to 1.5 on the same cards
+// with the matrix cores busy 94 % of the time at 1.43 GHz -- the power limit -- and this one 80 % at 1.6 GHz.
+// One term takes 0.46 to 0.49 ms, 1.0 PFLOP/s: with the products of a step down to a third, the 600 MB that
+// the ends of the tiles read and write (X in two terms, X^T) take 0.12 ms of their own, only part of which another
+// workgroup on the compute unit hides.  Steps on the way, same product in two terms: 1.45 ms with 128 x 128 tiles, 32 k per
+// stage and one stage ahead; 1.3 with 16 k and two ahead; 1.15 with 256 x 128 tiles; 1.07 with 256 x 256, reads between the
+// products and the ends' loads put before their stores.  More stages ahead, raised wave priority around the
+// products, and reads gathered into the first half of a stage changed nothing or cost 1 to 10 %.
 template <uint32_t TR, uint32_t TC, uint32_t Terms> struct Product {
     static constexpr uint32_t kKb = Terms == 1 || TR == 64 ? 2 : 1;                // k blocks per stage
     static constexpr uint32_t kBufs = 3;                                      // stages in LDS: one computed on, two on their way
@@ -173,98 +243,129 @@ template <uint32_t TR, uint32_t TC, uint32_t Terms> struct Product {
     static constexpr uint32_t kHalfQ = TC / 32 * kKb * Terms;
     static constexpr uint32_t kStage = (kHalfP + kHalfQ) * kBlk;              // elements per stage
     static constexpr uint32_t kLoads = (kHalfP + kHalfQ) / 4;                 // per wavefront and stage
+    static constexpr uint32_t kWaves = TR * TC > 256 * 128 ? 1 : 2;           // wavefronts per SIMD the registers are divided for
     static constexpr uint32_t kNR = TR / 64, kNC = TC / 64;                   // 32-blocks per wavefront
     static_assert(kHalfP % 4 == 0 && kHalfQ % 4 == 0, "a load instruction of four wavefronts stays within one operand");
 
     // `Swap`: lanes hold rows of P (four consecutive rows of Q each); else rows of Q
     template <bool Swap>
-    static __device__ __forceinline__ void run(const half_t *p, const half_t *q, uint32_t k_blocks_stored, uint32_t k_blocks,
+    static __device__ __forceinline__ void run(const half_t *p, const half_t *q, uint64_t p_plane, uint64_t q_plane, uint32_t k_blocks_stored, uint32_t stages,
                                                half_t *lds, v16f (&acc)[kNR][kNC]) {
         const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t wr = wave >> 1, wc = wave & 1;
-        const uint64_t row_step = (uint64_t)k_blocks_stored * 2 * kBlk;
+        const uint64_t row_step = (uint64_t)k_blocks_stored * kBlk;
+        auto load_part = [&](uint32_t kb0, uint32_t buf, uint32_t n) {
+            const uint32_t at = n * 4 + wave;
+            const bool second = n * 4 >= kHalfP;
+            const uint32_t in = second ? at - kHalfP : at;
+            const uint32_t rb = in / (kKb * Terms), rest = in % (kKb * Terms);
+            const half_t *from = (second ? q : p) + rb * row_step + (uint64_t)(kb0 + rest / Terms) * kBlk + (rest % Terms ? pick(second, q_plane, p_plane) : 0) + lane * 8;
+            __builtin_amdgcn_global_load_lds((const FSTX_GLOBAL void *)from, (FSTX_LDS void *)(lds + buf * kStage + at * kBlk), 16, 0, 0);
+        };
         auto load_stage = [&](uint32_t kb0, uint32_t buf) {
 #pragma unroll
-            for (uint32_t n = 0; n < kLoads; ++n) {
-                const uint32_t at = n * 4 + wave;
-                const bool second = n * 4 >= kHalfP;
-                const uint32_t in = second ? at - kHalfP : at;
-                const uint32_t rb = in / (kKb * Terms), rest = in % (kKb * Terms);
-                const half_t *from = (second ? q : p) + rb * row_step + (uint64_t)(kb0 + rest / Terms) * 2 * kBlk + (rest % Terms) * kBlk + lane * 8;
-                __builtin_amdgcn_global_load_lds((const FSTX_GLOBAL void *)from, (FSTX_LDS void *)(lds + buf * kStage + at * kBlk), 16, 0, 0);
-            }
+            for (uint32_t n = 0; n < kLoads; ++n) load_part(kb0, buf, n);
         };
-        v8h pf[kKb][kNR][Terms], qf[kKb][kNC][Terms];
-        auto fetch = [&](uint32_t buf) {
+        struct Fragments {
+            v8h p[kKb][kNR][Terms], q[kKb][kNC][Terms];
+        };
+        // A stage's LDS reads and its products, numbered: reads in the order in which products want them
+        constexpr uint32_t kReads = kKb * Terms * (kNR + kNC), kPerKb = (Terms == 1 ? 1 : 3) * kNR * kNC, kProducts = kKb * kPerKb;
+        auto read = [&](const half_t *base, Fragments &f, uint32_t r) {
+            const uint32_t kb = r / (Terms * (kNR + kNC)), m = r / (kNR + kNC) % Terms, i = r % (kNR + kNC);
+            if (i < kNR) f.p[kb][i][m] = *(const v8h *)(base + (((wr * kNR + i) * kKb + kb) * Terms + m) * kBlk);
+            else f.q[kb][i - kNR][m] = *(const v8h *)(base + (kHalfP + ((wc * kNC + i - kNR) * kKb + kb) * Terms + m) * kBlk);
+        };
+        auto product = [&](const Fragments &f, uint32_t n) {
+            const uint32_t kb = n / kPerKb, kind = n % kPerKb / (kNR * kNC), i = n / kNC % kNR, j = n % kNC;
+            const uint32_t mp = kind == 2, mq = kind == 1; // h h, h l, l h
+            acc[i][j] = Swap ? __builtin_amdgcn_mfma_f32_32x32x16_f16(f.q[kb][j][mq], f.p[kb][i][mp], acc[i][j], 0, 0, 0)
+                             : __builtin_amdgcn_mfma_f32_32x32x16_f16(f.p[kb][i][mp], f.q[kb][j][mq], acc[i][j], 0, 0, 0);
+        };
+        auto fetch = [&](uint32_t buf, Fragments &f) {
             const half_t *base = lds + buf * kStage + lane * 8;
 #pragma unroll
-            for (uint32_t kb = 0; kb < kKb; ++kb)
-#pragma unroll
-                for (uint32_t m = 0; m < Terms; ++m) {
-#pragma unroll
-                    for (uint32_t i = 0; i < kNR; ++i) pf[kb][i][m] = *(const v8h *)(base + (((wr * kNR + i) * kKb + kb) * Terms + m) * kBlk);
-#pragma unroll
-                    for (uint32_t j = 0; j < kNC; ++j) qf[kb][j][m] = *(const v8h *)(base + (kHalfP + ((wc * kNC + j) * kKb + kb) * Terms + m) * kBlk);
-                }
+            for (uint32_t r = 0; r < kReads; ++r) read(base, f, r);
         };
-        auto multiply = [&]() {
+        auto multiply = [&](const Fragments &f) {
 #pragma unroll
-            for (uint32_t kb = 0; kb < kKb; ++kb)
-#pragma unroll
-                for (int sum = 0; sum < (int)Terms; ++sum)
-#pragma unroll
-                    for (int m = 0; m <= sum; ++m)
-#pragma unroll
-                        for (uint32_t i = 0; i < kNR; ++i)
-#pragma unroll
-                            for (uint32_t j = 0; j < kNC; ++j)
-                                acc[i][j] = Swap ? __builtin_amdgcn_mfma_f32_32x32x16_f16(qf[kb][j][m], pf[kb][i][sum - m], acc[i][j], 0, 0, 0)
-                                                 : __builtin_amdgcn_mfma_f32_32x32x16_f16(pf[kb][i][m], qf[kb][j][sum - m], acc[i][j], 0, 0, 0);
+            for (uint32_t n = 0; n < kProducts; ++n) product(f, n);
         };
-        constexpr uint32_t kAhead = kBufs - 1;
-        const uint32_t stages = k_blocks / kKb;
-        for (uint32_t s = 0; s < kAhead && s < stages; ++s) load_stage(s * kKb, s);
-        uint32_t s = 0, buf = 0;
-        for (; s + kAhead < stages; ++s) {
-            // This wavefront's loads of the stage have landed (those of the next one may be on their way) and its
-            // reads of the stage before are done; behind the barrier that holds for all four.
-            constexpr uint32_t kLeft = (kAhead - 1) * kLoads;
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
-            fetch(buf);
-            load_stage((s + kAhead) * kKb, buf == 0 ? kBufs - 1 : buf - 1); // where the stage before was
-            multiply();
-            buf = buf + 1 == kBufs ? 0 : buf + 1;
+        auto after = [&](uint32_t buf) { return buf + 1 == kBufs ? 0 : buf + 1; };
+        for (uint32_t s = 0; s < kBufs && s < stages; ++s) load_stage(s * kKb, s);
+        Fragments even, odd;
+        if (stages < kBufs) wait_and_meet<0>();
+        else wait_and_meet<(kBufs - 1) * kLoads>();
+        fetch(0, even);
+        uint32_t buf = 0; // of the stage in registers
+        // One turn: the stage in `now` is multiplied while the next one is read from LDS into `next` and the
+        // one kBufs further on its way to where the stage in `now` was.  Before that, this wavefront's loads of
+        // the next stage have landed (kBufs - 2 later ones may be on their way) and its reads of `now` are done; behind
+        // the barrier that holds for all four.
+        auto turn = [&](uint32_t s, const Fragments &now, Fragments &next) {
+            wait_and_meet<(kBufs - 2) * kLoads>();
+            const half_t *base = lds + after(buf) * kStage + lane * 8;
+#pragma unroll
+            for (uint32_t r = 0; r < kReads; ++r) { // reads and loads in between the products
+                read(base, next, r);
+                if (r * kLoads / kReads != (r + 1) * kLoads / kReads) load_part((s + kBufs) * kKb, buf, r * kLoads / kReads);
+#pragma unroll
+                for (uint32_t n = r * kProducts / kReads; n < (r + 1) * kProducts / kReads; ++n) product(now, n);
+                __builtin_amdgcn_sched_barrier(0); // left alone, the compiler gathers the reads behind the products
+            }
+            buf = after(buf);
+        };
+        uint32_t s = 0;
+        for (; s + kBufs + 1 < stages; s += 2) {
+            turn(s, even, odd);
+            turn(s + 1, odd, even);
         }
-        for (; s < stages; ++s) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            fetch(buf);
-            multiply();
-            buf = buf + 1 == kBufs ? 0 : buf + 1;
+        for (;; ++s) { // the last stages: at most kBufs + 1 of them, the registers changing hands by copy
+            if (s + 1 == stages) break;
+            wait_and_meet<0>();
+            fetch(after(buf), odd);
+            if (s + kBufs < stages) load_stage((s + kBufs) * kKb, buf);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(even);
+            buf = after(buf);
+            even = odd;
         }
+        multiply(even);
     }
 };
 
+// Elements of one term of a matrix of so many blocks of 16 rows and columns
+__device__ __forceinline__ uint64_t plane_of(uint32_t row_blocks, uint32_t col_blocks) { return (uint64_t)row_blocks * col_blocks * 256; }
+
 // Where a lane's four values 4g..4g+3 of a 32 x 32 block lie in an operand: row block `rb`, columns 32 cb + 8g + 4 (lane / 32)..+3
 __device__ __forceinline__ uint64_t quad_at(uint32_t rb, uint32_t cb, uint32_t k_blocks_stored, uint32_t g, uint32_t lane) {
-    return ((uint64_t)rb * k_blocks_stored + 2 * cb + (g >> 1)) * 2 * kBlk + ((g & 1) * 32 + (lane & 31)) * 8 + 4 * (lane >> 5);
+    return ((uint64_t)rb * k_blocks_stored + 2 * cb + (g >> 1)) * kBlk + ((g & 1) * 32 + (lane & 31)) * 8 + 4 * (lane >> 5);
 }
 
-__device__ __forceinline__ v16f load_block(const half_t *m, uint32_t rb, uint32_t cb, uint32_t k_blocks_stored, uint32_t lane, bool both) {
-    v16f out;
+// What a lane holds of a 32 x 32 block as it is stored, and its value
+struct RawBlock {
+    v4h h[4], l[4];
+};
+__device__ __forceinline__ RawBlock load_block(const half_t *m, uint64_t plane, uint32_t rb, uint32_t cb, uint32_t k_blocks_stored, uint32_t lane, bool both) {
+    RawBlock out;
 #pragma unroll
     for (uint32_t g = 0; g < 4; ++g) {
         const half_t *at = m + quad_at(rb, cb, k_blocks_stored, g, lane);
-        const v4h h = *(const FSTX_GLOBAL v4h *)at;
-        v4h l = {};
-        if (both) l = *(const FSTX_GLOBAL v4h *)(at + kBlk);
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) out[4 * g + e] = (float)h[e] + (float)l[e];
+        out.h[g] = *(const FSTX_GLOBAL v4h *)at;
+        out.l[g] = v4h{};
+        if (both) out.l[g] = *(const FSTX_GLOBAL v4h *)(at + plane);
     }
     return out;
 }
+__device__ __forceinline__ v16f value_of(const RawBlock &b) {
+    v16f out;
+#pragma unroll
+    for (uint32_t r = 0; r < 16; ++r) out[r] = (float)b.h[r / 4][r % 4] + (float)b.l[r / 4][r % 4];
+    return out;
+}
 
-__device__ __forceinline__ void store_block(half_t *m, uint32_t rb, uint32_t cb, uint32_t k_blocks_stored, uint32_t lane, const half_t (&h)[16],
-                                            const half_t (&l)[16]) {
+__device__ __forceinline__ void store_block(half_t *m, uint64_t plane, uint32_t rb, uint32_t cb, uint32_t k_blocks_stored, uint32_t lane, const half_t (&h)[16],
+                                            const half_t (&l)[16], bool both) {
 #pragma unroll
     for (uint32_t g = 0; g < 4; ++g) {
         half_t *at = m + quad_at(rb, cb, k_blocks_stored, g, lane);
@@ -275,7 +376,7 @@ __device__ __forceinline__ void store_block(half_t *m, uint32_t rb, uint32_t cb,
             vl[e] = l[4 * g + e];
         }
         *(FSTX_GLOBAL v4h *)at = vh;
-        *(FSTX_GLOBAL v4h *)(at + kBlk) = vl;
+        if (both) *(FSTX_GLOBAL v4h *)(at + plane) = vl;
     }
 }
 
@@ -305,12 +406,51 @@ __device__ __forceinline__ void exchange(const half_t (&in)[16], half_t (&out)[1
     for (uint32_t r = 0; r < 16; ++r) out[r] = (half_t)d[r];
 }
 
+// X and X^T from G: a wavefront takes a 32 x 32 block, its lanes along the side along which memory runs.
+__global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const float eps, const uint32_t low_term) {
+    const uint32_t ji = job_of(t, blockIdx.x);
+    const Job job = fetch_job(t, ji);
+    const uint32_t lane = threadIdx.x & 63;
+    double sum = 0;
+    for (uint32_t i = lane; i < job.n_partials; i += 64) sum += job.partials[i];
+    const float norm = (float)sqrt(wave_sum(sum));
+    const float factor = job.scale / (norm + eps);
+
+    const View g = view_of(job);
+    const uint32_t p_blocks = pad_to(job.p, kPadP) / 16, q_blocks = pad_to(job.q, kPadQ) / 16;
+    const uint32_t across = (g.x_cols ? q_blocks : p_blocks) / 2, down = (g.x_cols ? p_blocks : q_blocks) / 2;
+    const uint32_t blk = (blockIdx.x - t.first[ji]) * 4 + threadIdx.x / 64;
+    if (blk >= across * down) return;
+    const uint32_t rb = blk / across, cb = blk - rb * across;
+    const uint32_t col = cb * 32 + (lane & 31);
+    v16f v;
+#pragma unroll
+    for (uint32_t r = 0; r < 16; ++r) {
+        const uint32_t row = rb * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+        v[r] = row < g.rows && col < g.cols ? load_elem(job.src, (uint64_t)row * g.row_stride + (uint64_t)col * g.col_stride, job.type) * factor : 0.0f;
+    }
+    half_t h[16], l[16], ht[16], lt[16];
+    split(v, h, l);
+    exchange(h, ht, lane);
+    exchange(l, lt, lane);
+    const uint64_t plane = plane_of(p_blocks, q_blocks);
+    // X's second term is always wanted (a X keeps both), X^T's where the first product has two terms
+    if (g.x_cols) {
+        store_block(job.xt0, plane, cb, rb, p_blocks, lane, h, l, low_term);
+        store_block(job.x, plane, rb, cb, q_blocks, lane, ht, lt, true);
+    } else {
+        store_block(job.x, plane, cb, rb, q_blocks, lane, h, l, true);
+        store_block(job.xt0, plane, rb, cb, p_blocks, lane, ht, lt, low_term);
+    }
+}
+
 enum Phase : uint32_t { kGram, kPoly, kApply, kLast };
 
 struct Coefficients {
-    float own, product; // result = own * (what is there) + product * (sum of the products)
-    uint32_t current;   // which of xt[] is the current one
-    uint32_t both;      // whether "what is there" is taken with both terms
+    float own, product;  // result = own * (what is there) + product * (sum of the products)
+    uint32_t current;    // which of xt0, xt1 is the current one
+    uint32_t own_both;   // "what is there" is taken with both its terms
+    uint32_t next_both;  // the next step's products want both terms of X^T
 };
 
 // Tiles of a symmetric matrix that reach on or below the diagonal, row by row: row i has kAspect (i + 1) of
@@ -323,86 +463,190 @@ template <uint32_t kAspect> __device__ __forceinline__ void triangle(uint32_t t,
     j = t - triangle_tiles<kAspect>(i);
 }
 
-template <uint32_t kPhase, uint32_t TR, uint32_t TC, uint32_t Terms>
-__global__ __launch_bounds__(256, 2) void newton_schulz_kernel(const uint32_t dies_log2, const Jobs t, const Coefficients c) {
-    typedef Product<TR, TC, Terms> Prod;
-    constexpr uint32_t kNR = Prod::kNR, kNC = Prod::kNC;
-    __shared__ __attribute__((aligned(1024))) half_t lds[Prod::kBufs * Prod::kStage];
-    const uint32_t ji = job_of(t, blockIdx.x);
-    const Job &job = t.job[ji];
-    const uint32_t pt = (job.p + TR - 1) / TR, qt = (job.q + TC - 1) / TC;
-    const uint32_t p_blocks = pad_to(job.p, kPad) / 16, q_blocks = pad_to(job.q, kPad) / 16; // as stored
-    constexpr bool kSymmetric = kPhase == kGram || kPhase == kPoly;
-    uint32_t tile, ti, tj;
-    if (!fstx_gather::tile_for_die(blockIdx.x - t.first[ji], kSymmetric ? triangle_tiles<TR / TC>(pt) : pt * qt, dies_log2, tile)) return;
-    if (kSymmetric) {
+// own x + product v to rows first + 0..3, 8..11, 16..19, 24..27 of the destination, one column per lane
+template <typename T>
+__device__ __forceinline__ void store_rows(char *at, uint32_t col, uint64_t pitch, uint32_t first, uint32_t rows, const v16f &x, const v16f &v, float own,
+                                           float product) {
+    FSTX_GLOBAL char *to = (FSTX_GLOBAL char *)at + (uint64_t)col * sizeof(T);
+#pragma unroll
+    for (uint32_t r = 0; r < 16; ++r) {
+        const uint32_t row = 8 * (r / 4) + r % 4;
+        if (first + row < rows) *(FSTX_GLOBAL T *)(to + row * pitch) = (T)(own * x[r] + product * v[r]);
+    }
+}
+
+// What is there already where block (rb, cb) of a product goes: A's block, or X's
+template <uint32_t kPhase>
+__device__ __forceinline__ RawBlock own_block(const Job &job, const Coefficients &c, uint32_t rb, uint32_t cb, uint32_t lane) {
+    const uint32_t p_blocks = pad_to(job.p, kPadP) / 16, q_blocks = pad_to(job.q, kPadQ) / 16; // as stored
+    if constexpr (kPhase == kGram) {
+        return RawBlock{};
+    } else if constexpr (kPhase == kLast) {
+        const bool flipped = job.flipped;
+        return load_block(pick<const half_t *>(flipped, job.x, pick(c.current, job.xt1, job.xt0)), plane_of(p_blocks, q_blocks), pick(flipped, rb, cb), pick(flipped, cb, rb),
+                          pick(flipped, q_blocks, p_blocks), lane, c.own_both);
+    } else {
+        return load_block(kPhase == kPoly ? job.a : job.x, plane_of(p_blocks, kPhase == kPoly ? p_blocks : q_blocks), rb, cb,
+                          kPhase == kPoly ? p_blocks : q_blocks, lane, c.own_both);
+    }
+}
+
+// What becomes of one 32 x 32 block of a product. `v` is laid out with lanes along rows (the transposed
+// product), in the last step of a matrix that is not flipped with lanes along columns.
+template <uint32_t kPhase, uint32_t Terms>
+__device__ __forceinline__ void finish_block(const Job &job, const Coefficients &c, uint32_t rb, uint32_t cb, v16f v, const RawBlock &there, uint32_t lane) {
+    const uint32_t p_blocks = pad_to(job.p, kPadP) / 16, q_blocks = pad_to(job.q, kPadQ) / 16;
+    if constexpr (kPhase == kLast) {
+        // lanes run along the contiguous side of the destination: 64 or 128 contiguous bytes per row
+        const bool flipped = job.flipped;
+        const uint32_t along = pick(flipped, rb, cb) * 32 + (lane & 31), first = pick(flipped, cb, rb) * 32 + 4 * (lane >> 5);
+        const uint32_t rows = pick(flipped, job.q, job.p), cols = pick(flipped, job.p, job.q);
+        if (along >= cols) return;
+        const float own = c.own / job.scale, product = c.product / job.scale; // (powers of two)
+        const v16f x = value_of(there);
+        char *at = job.dst + (uint64_t)first * job.dst_pitch;
+        if (job.type == FSTX_F32) store_rows<float>(at, along, job.dst_pitch, first, rows, x, v, own, product);
+        else if (job.type == FSTX_BF16) store_rows<__bf16>(at, along, job.dst_pitch, first, rows, x, v, own, product);
+        else store_rows<half_t>(at, along, job.dst_pitch, first, rows, x, v, own, product);
+    } else {
+        if constexpr (kPhase == kGram) {
+            v *= c.product / (job.scale * job.scale);
+        } else {
+            const v16f own = value_of(there);
+#pragma unroll
+            for (uint32_t r = 0; r < 16; ++r) v[r] = c.own * own[r] + c.product * v[r];
+        }
+        half_t h[16], l[16], ht[16], lt[16];
+        split(v, h, l);
+        half_t *to = kPhase == kGram ? job.a : kPhase == kPoly ? job.b : job.x;
+        const uint64_t plane = plane_of(p_blocks, kPhase == kApply ? q_blocks : p_blocks);
+        store_block(to, plane, rb, cb, kPhase == kApply ? q_blocks : p_blocks, lane, h, l, kPhase == kApply || Terms == 2);
+        if (kPhase == kApply || cb != rb) {
+            const bool both = kPhase == kApply ? c.next_both : Terms == 2;
+            exchange(h, ht, lane);
+            if (both) exchange(l, lt, lane);
+            store_block(kPhase == kApply ? pick(c.current, job.xt0, job.xt1) : to, plane, cb, rb, p_blocks, lane, ht, lt, both);
+        }
+    }
+}
+
+template <uint32_t kPhase> __host__ __device__ constexpr bool symmetric() { return kPhase == kGram || kPhase == kPoly; }
+
+template <uint32_t kPhase, uint32_t TR, uint32_t TC> __host__ __device__ inline uint32_t tiles_of(uint32_t p, uint32_t q) {
+    const uint32_t pt = (p + TR - 1) / TR, qt = (q + TC - 1) / TC;
+    return symmetric<kPhase>() ? triangle_tiles<TR / TC>(pt) : pt * qt;
+}
+
+template <uint32_t kPhase, uint32_t TR, uint32_t TC>
+__device__ __forceinline__ void place_of(const Job &job, uint32_t tile, uint32_t &ti, uint32_t &tj) {
+    if constexpr (symmetric<kPhase>()) {
         triangle<TR / TC>(tile, ti, tj);
     } else { // columns of up to eight tiles, so that the tiles at work share both operands
+        const uint32_t pt = (job.p + TR - 1) / TR, qt = (job.q + TC - 1) / TC;
         const uint32_t group = tile / (8 * qt), first = group * 8, height = pt - first < 8 ? pt - first : 8;
         const uint32_t in = tile - group * 8 * qt;
         ti = first + in % height;
         tj = in / height;
     }
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t rb0 = ti * (TR / 32) + (wave >> 1) * kNR, cb0 = tj * (TC / 32) + (wave & 1) * kNC;
+}
 
-    v16f acc[kNR][kNC] = {};
-    if constexpr (kPhase == kGram) {
-        const uint64_t row = (uint64_t)q_blocks * 2 * kBlk;
-        Prod::template run<true>(job.x + ti * (TR / 32) * row, job.x + tj * (TC / 32) * row, q_blocks, pad_to(job.q, kStepPad) / 16, lds, acc);
-    } else if constexpr (kPhase == kPoly) {
-        const uint64_t row = (uint64_t)p_blocks * 2 * kBlk;
-        Prod::template run<true>(job.a + ti * (TR / 32) * row, job.a + tj * (TC / 32) * row, p_blocks, pad_to(job.p, kStepPad) / 16, lds, acc);
+template <uint32_t kPhase, uint32_t TR, uint32_t TC, uint32_t Terms>
+__global__ __launch_bounds__(256, (Product<TR, TC, Terms>::kWaves)) void newton_schulz_kernel(const Jobs t, const Deal deal, const Coefficients c) {
+    typedef Product<TR, TC, Terms> Prod;
+    constexpr uint32_t kNR = Prod::kNR, kNC = Prod::kNC;
+    __shared__ __attribute__((aligned(1024))) half_t lds[Prod::kBufs * Prod::kStage];
+    const uint32_t ji = job_of(t, blockIdx.x);
+    const Job job = fetch_job(t, ji);
+    const uint32_t lb = blockIdx.x - t.first[ji], whole = deal.whole[ji];
+    const uint32_t whole_wgs = (whole + (1u << deal.dies_log2) - 1) >> deal.dies_log2 << deal.dies_log2;
+    uint32_t tile, piece = 0, part = 0;
+    const bool partial = lb >= whole_wgs;
+    if (!partial) {
+        if (!fstx_gather::tile_for_die(lb, whole, deal.dies_log2, tile)) return;
     } else {
-        const uint64_t row = (uint64_t)p_blocks * 2 * kBlk;
-        const half_t *p = job.b + ti * (TR / 32) * row, *q = job.xt[c.current] + tj * (TC / 32) * row;
-        if (kPhase == kLast && !job.flipped) Prod::template run<false>(p, q, p_blocks, pad_to(job.p, kStepPad) / 16, lds, acc);
-        else Prod::template run<true>(p, q, p_blocks, pad_to(job.p, kStepPad) / 16, lds, acc);
+        piece = lb - whole_wgs;
+        tile = whole + piece / deal.split;
+        part = piece % deal.split;
     }
+    uint32_t ti, tj;
+    place_of<kPhase, TR, TC>(job, tile, ti, tj);
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
+    // the operands' tiles, and the k that are summed here
+    const uint32_t stored = (kPhase == kGram ? pad_to(job.q, kPadQ) : pad_to(job.p, kPadP)) / 16;
+    const uint32_t stages = pad_to(kPhase == kGram ? job.q : job.p, kStepPad) / 16 / Prod::kKb;
+    const uint32_t from = partial ? (uint32_t)((uint64_t)stages * part / deal.split) : 0;
+    const uint32_t to = partial ? (uint32_t)((uint64_t)stages * (part + 1) / deal.split) : stages;
+    const half_t *left = kPhase == kGram ? job.x : kPhase == kPoly ? job.a : job.b;
+    const half_t *right = kPhase == kGram ? job.x : kPhase == kPoly ? job.a : pick(c.current, job.xt1, job.xt0);
+    const uint64_t row = (uint64_t)stored * kBlk, k0 = (uint64_t)from * Prod::kKb * kBlk;
+    const uint32_t p_blocks = pad_to(job.p, kPadP) / 16, q_blocks = pad_to(job.q, kPadQ) / 16;
+    const uint64_t left_plane = plane_of(p_blocks, kPhase == kGram ? q_blocks : p_blocks);
+    const uint64_t right_plane = plane_of(p_blocks, kPhase == kPoly ? p_blocks : q_blocks);
+    left += ti * (TR / 32) * row + k0;
+    right += tj * (TC / 32) * row + k0;
+    v16f acc[kNR][kNC] = {};
+    if (kPhase == kLast && !job.flipped) Prod::template run<false>(left, right, left_plane, right_plane, stored, to - from, lds, acc);
+    else Prod::template run<true>(left, right, left_plane, right_plane, stored, to - from, lds, acc);
+
+    if (partial) {
+        float *out = deal.sums + ((uint64_t)deal.slot[ji] + piece) * (TR * TC) + wave * (kNR * kNC * 1024) + lane * 4;
 #pragma unroll
-    for (uint32_t i = 0; i < kNR; ++i)
+        for (uint32_t i = 0; i < kNR; ++i)
 #pragma unroll
-        for (uint32_t j = 0; j < kNC; ++j) {
-            const uint32_t rb = rb0 + i, cb = cb0 + j;
-            if (kSymmetric && cb > rb) continue; // written as the mirror of (cb, rb)
-            v16f v = acc[i][j];
-            if constexpr (kPhase == kLast) {
-                // lanes run along the contiguous side of the destination: 64 or 128 contiguous bytes per row
-                const v16f x = job.flipped ? load_block(job.x, rb, cb, q_blocks, lane, c.both) : load_block(job.xt[c.current], cb, rb, p_blocks, lane, c.both);
-                const uint32_t along = (job.flipped ? rb : cb) * 32 + (lane & 31);
-                const uint32_t rows = job.flipped ? job.q : job.p, cols = job.flipped ? job.p : job.q;
-                const float back = 1.0f / job.scale;
-                if (along < cols)
+            for (uint32_t j = 0; j < kNC; ++j)
 #pragma unroll
-                    for (uint32_t r = 0; r < 16; ++r) {
-                        const uint32_t row = (job.flipped ? cb : rb) * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-                        if (row >= rows) continue;
-                        const float out = (c.own * x[r] + c.product * v[r]) * back;
-                        char *at = job.dst + (uint64_t)row * job.dst_pitch;
-                        if (job.type == FSTX_F32) ((FSTX_GLOBAL float *)at)[along] = out;
-                        else if (job.type == FSTX_BF16) ((FSTX_GLOBAL __bf16 *)at)[along] = (__bf16)out;
-                        else ((FSTX_GLOBAL half_t *)at)[along] = (half_t)out;
-                    }
-                continue;
-            }
-            if constexpr (kPhase == kGram) {
-                v *= c.product / (job.scale * job.scale);
-            } else {
-                const v16f own = kPhase == kPoly ? load_block(job.a, rb, cb, p_blocks, lane, c.both) : load_block(job.x, rb, cb, q_blocks, lane, c.both);
+                for (uint32_t g = 0; g < 4; ++g)
+                    *(FSTX_GLOBAL v4f *)(out + (i * kNC + j) * 1024 + g * 256) =
+                        v4f{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        return;
+    }
+    // The blocks of one row of blocks: what is there already is read for the row after it before anything is
+    // written (a load behind a store would wait its turn), so that its latency is paid once.
+    const uint32_t rb0 = ti * (TR / 32) + (wave >> 1) * kNR, cb0 = tj * (TC / 32) + (wave & 1) * kNC;
+    RawBlock there[2][kNC];
+    auto fetch_row = [&](uint32_t i) {
 #pragma unroll
-                for (uint32_t r = 0; r < 16; ++r) v[r] = c.own * own[r] + c.product * v[r];
-            }
-            half_t h[16], l[16], ht[16], lt[16];
-            split(v, h, l);
-            half_t *to = kPhase == kGram ? job.a : kPhase == kPoly ? job.b : job.x;
-            store_block(to, rb, cb, kPhase == kApply ? q_blocks : p_blocks, lane, h, l);
-            if (kPhase == kApply || cb != rb) {
-                exchange(h, ht, lane);
-                exchange(l, lt, lane);
-                store_block(kPhase == kApply ? job.xt[c.current ^ 1] : to, cb, rb, p_blocks, lane, ht, lt);
-            }
+        for (uint32_t j = 0; j < kNC; ++j)
+            if (!symmetric<kPhase>() || cb0 + j <= rb0 + i) there[i % 2][j] = own_block<kPhase>(job, c, rb0 + i, cb0 + j, lane);
+    };
+    fetch_row(0);
+#pragma unroll
+    for (uint32_t i = 0; i < kNR; ++i) {
+        if (i + 1 < kNR) fetch_row(i + 1);
+#pragma unroll
+        for (uint32_t j = 0; j < kNC; ++j)
+            if (!symmetric<kPhase>() || cb0 + j <= rb0 + i) // above the diagonal: written as the mirror of (cb, rb)
+                finish_block<kPhase, Terms>(job, c, rb0 + i, cb0 + j, acc[i][j], there[i % 2][j], lane);
+    }
+}
+
+// The tiles whose sums came in pieces: a wavefront per 32 x 32 block adds them in order.
+template <uint32_t kPhase, uint32_t TR, uint32_t TC, uint32_t Terms>
+__global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Deal deal, const Coefficients c) {
+    typedef Product<TR, TC, Terms> Prod;
+    constexpr uint32_t kBlocks = TR / 32 * (TC / 32);
+    const uint32_t ji = job_of(t, blockIdx.x);
+    const Job job = fetch_job(t, ji);
+    const uint32_t lb = blockIdx.x - t.first[ji], in = lb % kBlocks, nth = lb / kBlocks;
+    uint32_t ti, tj;
+    place_of<kPhase, TR, TC>(job, deal.whole[ji] + nth, ti, tj);
+    const uint32_t ri = in / (TC / 32), ci = in % (TC / 32), rb = ti * (TR / 32) + ri, cb = tj * (TC / 32) + ci;
+    if (symmetric<kPhase>() && cb > rb) return;
+    const uint32_t wave = ri / Prod::kNR * 2 + ci / Prod::kNC, i = ri % Prod::kNR, j = ci % Prod::kNC;
+    const float *at = deal.sums + ((uint64_t)deal.slot[ji] + (uint64_t)nth * deal.split) * (TR * TC) +
+                      ((wave * Prod::kNR + i) * Prod::kNC + j) * 1024 + threadIdx.x * 4;
+    const RawBlock there = own_block<kPhase>(job, c, rb, cb, threadIdx.x);
+    v16f v = {};
+#pragma unroll 4
+    for (uint32_t s = 0; s < deal.split; ++s, at += TR * TC)
+#pragma unroll
+        for (uint32_t g = 0; g < 4; ++g) {
+            const v4f part = *(const FSTX_GLOBAL v4f *)(at + g * 256);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) v[4 * g + e] += part[e];
         }
+    finish_block<kPhase, Terms>(job, c, rb, cb, v, there, threadIdx.x);
 }
 
 // --------------------------------------------------------------- host side
@@ -418,7 +662,7 @@ inline bool empty(const fstx_orthogonalize_desc &d) { return d.rows == 0 || d.co
 struct Sides {
     uint64_t p, q, pp, qp;
     explicit Sides(const fstx_orthogonalize_desc &d)
-        : p(d.rows < d.cols ? d.rows : d.cols), q(d.rows < d.cols ? d.cols : d.rows), pp((p + kPad - 1) / kPad * kPad), qp((q + kPad - 1) / kPad * kPad) {}
+        : p(d.rows < d.cols ? d.rows : d.cols), q(d.rows < d.cols ? d.cols : d.rows), pp((p + kPadP - 1) / kPadP * kPadP), qp((q + kPadQ - 1) / kPadQ * kPadQ) {}
     uint64_t bytes() const { return (3 * pp * qp + 2 * pp * pp) * 2 * sizeof(half_t) + kPartials * sizeof(double); }
 };
 
@@ -451,156 +695,277 @@ int check(const fstx_orthogonalize_desc *descs, uint32_t n) {
     return 0;
 }
 
-// bf16 matrices take one term in the last step, the others two: each kind has launches of its own, so
-// that a matrix's result does not depend on what else is in the call.
-inline bool skip(const fstx_orthogonalize_desc &d, bool bf16) { return empty(d) || (d.type == FSTX_BF16) != bf16; }
+// Below kOneTermFrom a product's time is the latency of its few stages whatever their number of products: small matrices
+// keep two terms throughout, and matrices of all types share their launches ([1023, 257] and three smaller fp16 ones: 250 us
+// in two sets of launches, 160 in one).
+constexpr uint64_t kOneTermFrom = 512;
 
-// the descriptors [first, end) of one kind in one set of launches, and the workspace they take
-uint32_t next_chunk(const fstx_orthogonalize_desc *descs, uint32_t n, bool bf16, uint32_t first, uint64_t *bytes) {
-    uint32_t k = 0;
-    *bytes = 0;
-    for (uint32_t i = first; i < n; ++i) {
-        if (skip(descs[i], bf16)) continue;
-        const uint64_t need = Sides(descs[i]).bytes();
-        if (k == kMaxJobs || (k && *bytes + need > kChunkBytes)) return i;
-        *bytes += need;
-        ++k;
+// Which steps' products run on one term (bit k: step k).
+//
+// In the first steps a X is nearly all of the result: the singular values s of a matrix whose mean square
+// is 1 / p are small, and B X = (b s^2 + c s^4) X with them.  One term in the products of such a step, with both terms of X
+// in a X, is off by 2^-12 (|b| s^2 + |c| s^4) of the result, s^2 growing by a^2 per step; that model was met within
+// a factor of two on flat, decaying and spiked spectra (64-bit simulation with rounded operands).  A step takes one term
+// where it stays under 2^-12 for bf16 results (2^-9 of rounding), 2^-15 for fp16 (2^-12), 2^-21 for f32
+// (where 32-bit products themselves end at 2^-19 to 2^-17 on spiked spectra).
+// The LAST step of bf16 results takes one term too, in a X as well, so that the rounding of X enters with the slope of
+// the polynomial (below one there) and not with a and B separately: 4e-4 to 7e-4, against 1.7e-3 of rounding.
+uint64_t one_term_steps(const fstx_orthogonalize_desc &d, const float *coefficients, uint32_t steps) {
+    if ((d.rows < d.cols ? d.rows : d.cols) < kOneTermFrom) return 0;
+    const double budget = d.type == FSTX_BF16 ? 0x1p-12 : d.type == FSTX_F16 ? 0x1p-15 : 0x1p-21;
+    double s2 = 1.0 / (double)(d.rows < d.cols ? d.rows : d.cols);
+    uint64_t mask = 0;
+    for (uint32_t k = 0; k < steps; ++k) {
+        const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
+        if (0x1p-12 * (fabs(b) * s2 + fabs(c) * s2 * s2) <= budget && k + 1 < steps) mask |= 1ull << k;
+        s2 = s2 * a * a < 1.0 ? s2 * a * a : 1.0;
     }
-    return n;
+    if (d.type == FSTX_BF16) mask |= 1ull << (steps - 1);
+    return mask;
 }
 
 inline float power_of_two_below(double v) { return (float)ldexp(1.0, (int)floor(log2(v))); }
 
-// Workgroups a launch needs before larger tiles are taken: below that most of the 256 compute units would idle.
-constexpr uint64_t kLargeTiles = 200;
+// What the tile sizes cost, measured (microseconds): a launch and the ends of a workgroup; 16 k of one workgroup when
+// kResident share a compute unit, per workgroup, and when it is alone there.
+template <uint32_t TR, uint32_t TC, uint32_t Terms> struct Cost;
+#define FSTX_COST(TR, TC, TERMS, RESIDENT, FIXED, SHARED, ALONE)                                                     \
+    template <> struct Cost<TR, TC, TERMS> {                                                                         \
+        static constexpr uint32_t kResident = RESIDENT;                                                              \
+        static constexpr double kFixed = FIXED, kShared = SHARED, kAlone = ALONE;                                    \
+    };
+FSTX_COST(64, 64, 1, 6, 2.5, 0.057, 0.08)
+FSTX_COST(64, 64, 2, 3, 2.5, 0.12, 0.15)
+FSTX_COST(128, 128, 1, 3, 3.5, 0.165, 0.20)
+FSTX_COST(128, 128, 2, 3, 3.5, 0.355, 0.36)
+FSTX_COST(256, 128, 1, 2, 5.0, 0.275, 0.35)
+FSTX_COST(256, 128, 2, 2, 5.0, 0.630, 0.70)
+FSTX_COST(256, 256, 1, 1, 8.0, 0.545, 0.545)
+FSTX_COST(256, 256, 2, 1, 8.0, 1.230, 1.230)
+#undef FSTX_COST
 
 struct Launcher {
     Jobs t;
+    Deal d;
     uint32_t n = 0;
-    hipStream_t stream;
+    uint32_t grid = 0;       // of the last deal
+    uint64_t sum_tiles = 0;  // tiles of partial sums it takes
+    hipStream_t stream = nullptr;
+    bool run = false;        // false: only plan, and note how much room partial sums take
+    uint64_t sum_bytes = 0;
 
-    template <uint32_t kPhase, uint32_t TR, uint32_t TC> uint64_t tiles() const {
-        uint64_t sum = 0;
-        for (uint32_t i = 0; i < n; ++i) sum += tiles_of<kPhase, TR, TC>(t.job[i]);
-        return sum;
-    }
-    template <uint32_t kPhase, uint32_t TR, uint32_t TC> static uint64_t tiles_of(const Job &j) {
-        const uint32_t pt = (j.p + TR - 1) / TR, qt = (j.q + TC - 1) / TC;
-        return kPhase == kGram || kPhase == kPoly ? triangle_tiles<TR / TC>(pt) : (uint64_t)pt * qt;
+    // Deals the tiles to workgroups.  Whole rounds take a tile each.  Tiles that are left over would keep a few compute
+    // units busy for the time of a whole tile while the others idle: they can be cut along k into pieces instead, as many
+    // as there is room for, at the price of a second launch that joins them.  Returns an estimate in microseconds.
+    template <uint32_t kPhase, uint32_t TR, uint32_t TC, uint32_t Terms> double deal() {
+        typedef Cost<TR, TC, Terms> cost;
+        uint64_t tiles = 0;
+        uint32_t blocks = ~0u, longest = 0; // of 16 k
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t k = pad_to(kPhase == kGram ? t.job[i].q : t.job[i].p, kStepPad) / 16;
+            tiles += tiles_of<kPhase, TR, TC>(t.job[i].p, t.job[i].q);
+            if (k < blocks) blocks = k;
+            if (k > longest) longest = k;
+        }
+        const uint32_t units = 32u << d.dies_log2;
+        auto rounds = [&](uint64_t workgroups) { // time of 16 k for so many workgroups
+            const uint64_t full = workgroups / (units * cost::kResident), rest = workgroups % (units * cost::kResident);
+            const double last = cost::kShared * (double)((rest + units - 1) / units);
+            return (double)full * cost::kResident * cost::kShared + (rest ? last > cost::kAlone ? last : cost::kAlone : 0.0);
+        };
+        double best = cost::kFixed + longest * rounds(tiles);
+        uint32_t split = 1;
+        uint64_t whole = tiles;
+        for (uint32_t room = units; room <= 2 * units; room += units) {
+            const uint64_t left = tiles % room;
+            uint64_t cut = left ? room / left : 1;
+            if (cut > blocks / 8) cut = blocks / 8; // eight blocks of 16 k at least
+            if (cut < 2) continue;
+            const double megabytes = (double)(left * cut) * TR * TC * sizeof(float) / 1e6;
+            const double time = 2 * cost::kFixed + longest * (rounds(tiles - left) + rounds(left * cut) / (double)cut) + 2.0 + 0.35 * megabytes;
+            if (time >= best) continue;
+            best = time;
+            split = (uint32_t)cut;
+            whole = tiles - left;
+        }
+        d.split = split;
+        uint64_t wgs = 0;
+        sum_tiles = 0;
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint64_t mine = tiles_of<kPhase, TR, TC>(t.job[i].p, t.job[i].q), w = mine < whole ? mine : whole;
+            whole -= w;
+            t.first[i] = (uint32_t)wgs;
+            d.whole[i] = (uint32_t)w;
+            d.slot[i] = (uint32_t)sum_tiles;
+            wgs += (w + (1u << d.dies_log2) - 1) >> d.dies_log2 << d.dies_log2;
+            wgs += (mine - w) * split;
+            sum_tiles += (mine - w) * split;
+        }
+        grid = wgs * 256 > 0xffffffffull ? 0 : (uint32_t)wgs;
+        return best;
     }
 
     template <uint32_t kPhase, uint32_t TR, uint32_t TC, uint32_t Terms> int launch(const Coefficients &c) {
-        const uint32_t dl = fstx_internal::dies_log2();
-        uint64_t grid = 0;
-        for (uint32_t i = 0; i < n; ++i) {
-            t.first[i] = (uint32_t)grid;
-            grid += (tiles_of<kPhase, TR, TC>(t.job[i]) + (1u << dl) - 1) >> dl << dl;
+        deal<kPhase, TR, TC, Terms>();
+        if (!run) {
+            const uint64_t bytes = sum_tiles * TR * TC * sizeof(float);
+            if (bytes > sum_bytes) sum_bytes = bytes;
+            return grid ? 0 : -FSTX_E_RANGE;
         }
-        if (grid * 256 > 0xffffffffull) return -FSTX_E_RANGE;
-        fstx_internal::Range range("fstx newton_schulz_kernel: phase %u, %u matrices, %llu tiles of %u x %u", kPhase, n, (unsigned long long)grid, TR, TC);
-        hipLaunchKernelGGL((newton_schulz_kernel<kPhase, TR, TC, Terms>), dim3((uint32_t)grid), dim3(256), 0, stream, dl, t, c);
-        return fstx_internal::check_launch("newton_schulz_kernel");
+        {
+            fstx_internal::Range range("fstx newton_schulz_kernel: phase %u, %u matrices, %u workgroups, tiles of %u x %u", kPhase, n, grid, TR, TC);
+            hipLaunchKernelGGL((newton_schulz_kernel<kPhase, TR, TC, Terms>), dim3(grid), dim3(256), 0, stream, t, d, c);
+            const int rc = fstx_internal::check_launch("newton_schulz_kernel");
+            if (rc < 0 || sum_tiles == 0) return rc;
+        }
+        uint32_t wgs = 0;
+        for (uint32_t i = 0; i < n; ++i) {
+            t.first[i] = wgs;
+            wgs += (tiles_of<kPhase, TR, TC>(t.job[i].p, t.job[i].q) - d.whole[i]) * (TR / 32) * (TC / 32);
+        }
+        fstx_internal::Range range("fstx join_pieces_kernel: phase %u, %u workgroups", kPhase, wgs);
+        hipLaunchKernelGGL((join_pieces_kernel<kPhase, TR, TC, Terms>), dim3(wgs), dim3(64), 0, stream, t, d, c);
+        return fstx_internal::check_launch("join_pieces_kernel");
     }
 
     template <uint32_t kPhase, uint32_t Terms> int phase(const Coefficients &c) {
-        if constexpr (kPhase == kApply || kPhase == kLast)
-            if (tiles<kPhase, 256, 128>() >= kLargeTiles) return launch<kPhase, 256, 128, Terms>(c);
-        return tiles<kPhase, 128, 128>() >= kLargeTiles ? launch<kPhase, 128, 128, Terms>(c) : launch<kPhase, 64, 64, Terms>(c);
+        const double t256 = deal<kPhase, 256, 256, Terms>(), t128 = deal<kPhase, 256, 128, Terms>(), t = deal<kPhase, 128, 128, Terms>(),
+                     small = deal<kPhase, 64, 64, Terms>();
+        if (small <= t && small <= t128 && small <= t256) return launch<kPhase, 64, 64, Terms>(c);
+        if (t <= t128 && t <= t256) return launch<kPhase, 128, 128, Terms>(c);
+        return t128 <= t256 ? launch<kPhase, 256, 128, Terms>(c) : launch<kPhase, 256, 256, Terms>(c);
     }
-    template <uint32_t kPhase> int phase(uint32_t terms, const Coefficients &c) {
-        if constexpr (kPhase == kApply) return phase<kPhase, 2>(c); // never the last step
-        else return terms == 1 ? phase<kPhase, 1>(c) : phase<kPhase, 2>(c);
+    template <uint32_t kPhase> int phase(bool one, const Coefficients &c) { return one ? phase<kPhase, 1>(c) : phase<kPhase, 2>(c); }
+
+    int steps(const float *coefficients, uint32_t count, uint64_t one_term) {
+        for (uint32_t step = 0; step < count; ++step) {
+            const float a = coefficients[3 * step], b = coefficients[3 * step + 1], c = coefficients[3 * step + 2];
+            // B is held times this: its entries stay below fp16's largest while singular values are below sqrt(2)
+            const float scale_b = power_of_two_below(30000.0 / (2.0 * fabs((double)b) + 4.0 * fabs((double)c) + 0.01));
+            const bool last = step + 1 == count, one = one_term >> step & 1;
+            const uint32_t current = step & 1, next_both = !last && !(one_term >> (step + 1) & 1);
+            int rc;
+            if ((rc = phase<kGram>(one, Coefficients{0, kScaleA, current, 0, 0})) < 0) return rc;
+            if ((rc = phase<kPoly>(one, Coefficients{b * scale_b / kScaleA, c * scale_b / (kScaleA * kScaleA), current, !one, 0})) < 0) return rc;
+            const Coefficients apply{a, 1.0f / scale_b, current, !last || !one, next_both};
+            if ((rc = last ? phase<kLast>(one, apply) : phase<kApply>(one, apply)) < 0) return rc;
+        }
+        return 0;
+    }
+
+    void add(const fstx_orthogonalize_desc &desc, char *at) {
+        const Sides s(desc);
+        const bool flipped = desc.rows > desc.cols;
+        Job &j = t.job[n++];
+        j = Job{};
+        j.src = static_cast<const char *>(desc.src);
+        j.dst = static_cast<char *>(desc.dst);
+        const uint64_t xb = s.pp * s.qp * 2 * sizeof(half_t), ab = s.pp * s.pp * 2 * sizeof(half_t);
+        j.x = reinterpret_cast<half_t *>(at);
+        j.xt0 = reinterpret_cast<half_t *>(at + xb);
+        j.xt1 = reinterpret_cast<half_t *>(at + 2 * xb);
+        j.a = reinterpret_cast<half_t *>(at + 3 * xb);
+        j.b = reinterpret_cast<half_t *>(at + 3 * xb + ab);
+        j.partials = reinterpret_cast<double *>(at + 3 * xb + 2 * ab);
+        j.x_row = flipped ? desc.src_col_stride : desc.src_row_stride;
+        j.x_col = flipped ? desc.src_row_stride : desc.src_col_stride;
+        j.dst_pitch = desc.dst_pitch * size_of(desc.type);
+        j.p = (uint32_t)s.p;
+        j.q = (uint32_t)s.q;
+        j.type = desc.type;
+        j.flipped = flipped;
+        // entries of X are at most about 1.2 (the spectral norm), their mean square is 1 / (p q) at first
+        const double mid = sqrt((double)s.p * (double)s.q);
+        j.scale = power_of_two_below(mid < 8192.0 ? mid : 8192.0);
+        const uint64_t parts = (s.p * s.q + 8191) / 8192;
+        j.n_partials = (uint32_t)(parts < kPartials ? parts : kPartials);
     }
 };
 
+// The matrices of one set of launches: those from `first` on that take one term in the same steps as `first` (so
+// that what a matrix is rounded to does not depend on what else is in the call), as many as fit.
+// Returns where the next set of that kind begins.
+uint32_t next_set(const fstx_orthogonalize_desc *descs, uint32_t n, const float *coefficients, uint32_t steps, uint32_t first, char *at, Launcher *set,
+                  uint64_t *bytes) {
+    const uint64_t kind = one_term_steps(descs[first], coefficients, steps);
+    *bytes = 0;
+    set->n = 0;
+    for (uint32_t k = 0; k < kMaxJobs; ++k) set->t.first[k] = 0xffffffffu;
+    for (uint32_t i = first; i < n; ++i) {
+        if (empty(descs[i]) || one_term_steps(descs[i], coefficients, steps) != kind) continue;
+        const uint64_t need = Sides(descs[i]).bytes();
+        if (set->n == kMaxJobs || (set->n && *bytes + need > kChunkBytes)) return i;
+        set->add(descs[i], at + *bytes);
+        *bytes += need;
+    }
+    return n;
+}
+
+// whether an earlier descriptor is of the same kind (and its sets have taken this one)
+bool taken(const fstx_orthogonalize_desc *descs, uint32_t i, const float *coefficients, uint32_t steps) {
+    const uint64_t kind = one_term_steps(descs[i], coefficients, steps);
+    for (uint32_t j = 0; j < i; ++j)
+        if (!empty(descs[j]) && one_term_steps(descs[j], coefficients, steps) == kind) return true;
+    return false;
+}
+
 } // namespace
 
-extern "C" int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *descs, uint32_t n) {
+extern "C" int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *descs, uint32_t n, const float *coefficients, uint32_t steps) {
     const int rc = check(descs, n);
     if (rc < 0) return rc;
+    if (steps < 1 || steps > kMaxSteps || !coefficients) return -FSTX_E_INVAL;
     uint64_t most = 0;
-    for (int bf16 = 0; bf16 < 2; ++bf16)
-        for (uint32_t i = 0; i < n;) {
+    for (uint32_t i = 0; i < n; ++i) {
+        if (empty(descs[i]) || taken(descs, i, coefficients, steps)) continue;
+        for (uint32_t first = i; first < n;) {
+            Launcher set;
+            set.d.dies_log2 = fstx_internal::dies_log2();
             uint64_t bytes;
-            i = next_chunk(descs, n, bf16, i, &bytes);
-            if (bytes > most) most = bytes;
+            const uint64_t kind = one_term_steps(descs[first], coefficients, steps);
+            first = next_set(descs, n, coefficients, steps, first, nullptr, &set, &bytes);
+            const int planned = set.steps(coefficients, steps, kind);
+            if (planned < 0) return planned;
+            if (bytes + set.sum_bytes > most) most = bytes + set.sum_bytes;
         }
+    }
     return (int64_t)most;
 }
 
 extern "C" int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t n, const float *coefficients, uint32_t steps, float eps,
                                   void *workspace, uint64_t workspace_bytes, void *stream) {
-    const int64_t need = fstx_orthogonalize_workspace(descs, n);
+    const int64_t need = fstx_orthogonalize_workspace(descs, n, coefficients, steps);
     if (need < 0) return (int)need;
-    if (steps < 1 || steps > kMaxSteps || !coefficients || !(eps >= 0)) return -FSTX_E_INVAL;
+    if (!(eps >= 0)) return -FSTX_E_INVAL;
     if (need && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (uint64_t)need)) return -FSTX_E_INVAL;
-    for (int bf16 = 0; bf16 < 2; ++bf16)
-        for (uint32_t i = 0; i < n;) {
+    for (uint32_t i = 0; i < n; ++i) {
+        if (empty(descs[i]) || taken(descs, i, coefficients, steps)) continue;
+        for (uint32_t first = i; first < n;) {
+            Launcher set;
+            set.d.dies_log2 = fstx_internal::dies_log2();
+            set.stream = static_cast<hipStream_t>(stream);
+            set.run = true;
             uint64_t bytes;
-            const uint32_t end = next_chunk(descs, n, bf16, i, &bytes);
-            Launcher run;
-            run.stream = static_cast<hipStream_t>(stream);
-            for (uint32_t k = 0; k < kMaxJobs; ++k) run.t.first[k] = 0xffffffffu;
-            char *at = static_cast<char *>(workspace);
-            for (; i < end; ++i) {
-                const fstx_orthogonalize_desc &d = descs[i];
-                if (skip(d, bf16)) continue;
-                const Sides s(d);
-                const bool flipped = d.rows > d.cols;
-                Job &j = run.t.job[run.n++];
-                j = Job{};
-                j.src = static_cast<const char *>(d.src);
-                j.dst = static_cast<char *>(d.dst);
-                const uint64_t xb = s.pp * s.qp * 2 * sizeof(half_t), ab = s.pp * s.pp * 2 * sizeof(half_t);
-                j.x = reinterpret_cast<half_t *>(at);
-                j.xt[0] = reinterpret_cast<half_t *>(at + xb);
-                j.xt[1] = reinterpret_cast<half_t *>(at + 2 * xb);
-                j.a = reinterpret_cast<half_t *>(at + 3 * xb);
-                j.b = reinterpret_cast<half_t *>(at + 3 * xb + ab);
-                j.partials = reinterpret_cast<double *>(at + 3 * xb + 2 * ab);
-                at += s.bytes();
-                j.x_row = flipped ? d.src_col_stride : d.src_row_stride;
-                j.x_col = flipped ? d.src_row_stride : d.src_col_stride;
-                j.dst_pitch = d.dst_pitch * size_of(d.type);
-                j.p = (uint32_t)s.p;
-                j.q = (uint32_t)s.q;
-                j.type = d.type;
-                j.flipped = flipped;
-                // entries of X are at most about 1.2 (the spectral norm), their mean square is 1 / (p q) at first
-                const double mid = sqrt((double)s.p * (double)s.q);
-                j.scale = power_of_two_below(mid < 8192.0 ? mid : 8192.0);
-                const uint64_t parts = (s.p * s.q + 16383) / 16384;
-                j.n_partials = (uint32_t)(parts < kPartials ? parts : kPartials);
-            }
-            if (run.n == 0) continue;
+            const uint64_t kind = one_term_steps(descs[first], coefficients, steps);
+            first = next_set(descs, n, coefficients, steps, first, static_cast<char *>(workspace), &set, &bytes);
+            set.d.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + bytes);
             uint64_t grid = 0;
-            for (uint32_t k = 0; k < run.n; ++k) {
-                run.t.first[k] = (uint32_t)grid;
-                grid += run.t.job[k].n_partials;
+            for (uint32_t k = 0; k < set.n; ++k) {
+                set.t.first[k] = (uint32_t)grid;
+                grid += set.t.job[k].n_partials;
             }
-            hipLaunchKernelGGL(sum_squares_kernel, dim3((uint32_t)grid), dim3(256), 0, run.stream, run.t);
+            hipLaunchKernelGGL(sum_squares_kernel, dim3((uint32_t)grid), dim3(256), 0, set.stream, set.t);
             int rc = fstx_internal::check_launch("sum_squares_kernel");
             if (rc < 0) return rc;
             grid = 0;
-            for (uint32_t k = 0; k < run.n; ++k) {
-                const uint64_t pp = pad_to(run.t.job[k].p, kPad), qp = pad_to(run.t.job[k].q, kPad);
-                run.t.first[k] = (uint32_t)grid;
-                grid += (pp / 32) * (qp / 16) * 2 / 4;
+            for (uint32_t k = 0; k < set.n; ++k) {
+                set.t.first[k] = (uint32_t)grid;
+                grid += (uint64_t)(pad_to(set.t.job[k].p, kPadP) / 32) * (pad_to(set.t.job[k].q, kPadQ) / 32) / 4;
             }
-            if (grid * 256 > 0xffffffffull) return -FSTX_E_RANGE;
-            hipLaunchKernelGGL(first_operands_kernel, dim3((uint32_t)grid), dim3(256), 0, run.stream, run.t, eps);
+            hipLaunchKernelGGL(first_operands_kernel, dim3((uint32_t)grid), dim3(256), 0, set.stream, set.t, eps, (uint32_t)!(kind & 1));
             if ((rc = fstx_internal::check_launch("first_operands_kernel")) < 0) return rc;
-            for (uint32_t step = 0; step < steps; ++step) {
-                const float a = coefficients[3 * step], b = coefficients[3 * step + 1], c = coefficients[3 * step + 2];
-                // B is held times this: its entries stay below fp16's largest while singular values are below sqrt(2)
-                const float scale_b = power_of_two_below(30000.0 / (2.0 * fabs((double)b) + 4.0 * fabs((double)c) + 0.01));
-                const bool last = step + 1 == steps;
-                const uint32_t terms = last && bf16 ? 1 : 2, current = step & 1, both = terms == 2;
-                if ((rc = run.phase<kGram>(terms, Coefficients{0, kScaleA, current, 1})) < 0) return rc;
-                if ((rc = run.phase<kPoly>(terms, Coefficients{b * scale_b / kScaleA, c * scale_b / (kScaleA * kScaleA), current, both})) < 0) return rc;
-                const Coefficients apply{a, 1.0f / scale_b, current, both};
-                if ((rc = last ? run.phase<kLast>(terms, apply) : run.phase<kApply>(terms, apply)) < 0) return rc;
-            }
+            if ((rc = set.steps(coefficients, steps, kind)) < 0) return rc;
         }
+    }
     return 0;
 }

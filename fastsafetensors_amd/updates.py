@@ -185,8 +185,9 @@ def orthogonalize(
     Returns new tensors of the updates' shapes and types, or fills ``outs`` (contiguous rows or
     contiguous columns; an update may be its own ``out``).  One tensor in, one tensor out; a sequence gives a list.
     The matrices of one call run together, so that small ones share launches.  All are checked before
-    anything runs.  Products are as accurate as 32-bit ones whatever the type; only the last step of a bf16 update
-    works on shorter operands, below what bf16 can tell apart.
+    anything runs.  The iterates are held in 22 bits and products are as accurate as 32-bit ones, except where
+    shorter operands (11 bits) cannot be told from that in a result of the update's type: in steps in which the
+    product is a small part of the sum, and in the last step of a bf16 update.
 
     The default coefficients leave singular values between 0.7 and 1.2, which is what an optimiser needs;
     appending a few ``(1.875, -1.25, 0.375)`` steps drives them to 1.  Coefficients must keep the
@@ -231,14 +232,15 @@ def orthogonalize(
         d.dst_pitch = _pitch(out, "out")
         d.src_row_stride, d.src_col_stride = g.stride()
         d.type = _FACTOR_TYPES[g.dtype]
-    try:
-        need = _native.orthogonalize_workspace(descs, len(mats))
-    except _native.NativeError as e:
-        raise ValueError(f"orthogonalize: outs overlap each other or other updates, or a size is out of range ({e})") from None
+    triples, steps = (_native.ctypes.c_float * len(flat))(*flat), len(flat) // 3
     with torch.cuda.device(device):
+        try:
+            need = _native.orthogonalize_workspace(descs, len(mats), triples, steps)
+        except _native.NativeError as e:
+            raise ValueError(f"orthogonalize: outs overlap each other or other updates, or a size is out of range ({e})") from None
         space = torch.empty(need, dtype=torch.uint8, device=device)
-        _native.orthogonalize(descs, len(mats), (_native.ctypes.c_float * len(flat))(*flat), len(flat) // 3, float(eps),
-                              space.data_ptr() if need else 0, need, torch.cuda.current_stream(device).cuda_stream)
+        _native.orthogonalize(descs, len(mats), triples, steps, float(eps), space.data_ptr() if need else 0, need,
+                              torch.cuda.current_stream(device).cuda_stream)
     if given:
         torch.autograd.graph.increment_version(outs)
     return outs[0] if single else outs

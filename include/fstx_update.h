@@ -53,8 +53,9 @@ int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, void *works
 
 /* dst = the nearest orthogonal matrix of src, approximated by `steps` Newton-Schulz steps:
  *   X = src / (|src|_F + eps);   per step (a, b, c):  A = X X^T,  X <- a X + (b A + c A A) X
- * with the shorter side as rows (orthogonal rows if rows <= cols, else orthogonal columns).  Products
- * are as accurate as 32-bit ones; sums are held in 32 bits, the norm in 64.  While the steps run the
+ * with the shorter side as rows (orthogonal rows if rows <= cols, else orthogonal columns).  Iterates are
+ * held in 22 bits and products as accurate as 32-bit ones, shorter operands only where a result of the
+ * type cannot tell; sums are held in 32 bits, the norm's in 64.  While the steps run the
  * iterates' singular values have to stay below about 2 (those of X start at 1 or less). */
 typedef struct fstx_orthogonalize_desc {
     void *dst;                              /* [rows, cols] of `type`, rows dst_pitch elements apart     */
@@ -66,8 +67,9 @@ typedef struct fstx_orthogonalize_desc {
     uint32_t reserved;
 } fstx_orthogonalize_desc;
 
-/* Bytes of workspace for these descriptors, or a negative status. */
-int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *descs, uint32_t n);
+/* Bytes of workspace for these descriptors and steps on the current device, or a negative status. */
+int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *descs, uint32_t n, const float *coefficients,
+                                     uint32_t steps);
 
 /* Any number of matrices; those that fit one set of launches together run together.  `coefficients`
  * (host memory) are a, b, c of each of the 1..64 steps.  No destination may overlap another

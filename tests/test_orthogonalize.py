@@ -16,22 +16,27 @@ def desc(dst=BASE, src=2 * BASE, rows=100, cols=300, pitch=None, strides=None, t
     return _native.FstxOrthogonalizeDesc(dst, src, rows, cols, cols if pitch is None else pitch, *(strides or (cols, 1)), type, 0)
 
 
+FIVE = (ctypes.c_float * 15)(*(3.4445, -4.775, 2.0315) * 5)
+
+
 def need(*descs):
-    return _native.lib().fstx_orthogonalize_workspace((_native.FstxOrthogonalizeDesc * len(descs))(*descs), len(descs))
+    return _native.lib().fstx_orthogonalize_workspace((_native.FstxOrthogonalizeDesc * len(descs))(*descs), len(descs), FIVE, 5)
 
 
 def size(p, q):
-    return (3 * p * q + 2 * p * p) * 4 + 2048  # X, two X^T, A and B in two terms; partial sums
+    return (3 * p * q + 2 * p * p) * 4 + 8192  # X, two X^T, A and B in two terms; partial sums of squares
 
 
 def test_workspace_sizes():
     assert need() == 0 and need(desc(rows=0)) == 0 and need(desc(cols=0)) == 0
-    assert need(desc()) == need(desc(rows=300, cols=100)) == size(128, 384)
-    assert need(desc(rows=1, cols=1)) == size(128, 128)
+    # operands padded to 256 x 128, and at most one round of workgroups' partial sums (512 tiles of 256 x 128)
+    for rows, cols, p, q in ((100, 300, 256, 384), (300, 100, 256, 384), (1, 1, 256, 128), (1000, 2500, 1024, 2560)):
+        got = need(desc(rows=rows, cols=cols))
+        assert size(p, q) <= got <= size(p, q) + 512 * 256 * 128 * 4
     small = [desc(dst=BASE + (i << 20), src=2 * BASE + (i << 20)) for i in range(50)]
-    assert need(*small) == 20 * size(128, 384)  # twenty at a time
+    assert 20 * size(256, 384) <= need(*small) < 21 * size(256, 384) + 512 * 256 * 128 * 4  # twenty at a time
     large = [desc(dst=(i + 1) << 36, src=(i + 100) << 36, rows=16384, cols=16384) for i in range(3)]
-    assert need(*large) == size(16384, 16384)   # one at a time
+    assert size(16384, 16384) <= need(*large) < 2 * size(16384, 16384)   # one at a time
 
 
 @pytest.mark.parametrize("bad,code", [
@@ -53,7 +58,8 @@ def test_overlaps():
 
 def test_steps_eps_and_workspace_are_checked():
     fn, arr, c = _native.lib().fstx_orthogonalize, (_native.FstxOrthogonalizeDesc * 1)(desc()), (ctypes.c_float * 3)(1.5, -0.5, 0.0)
-    n = need(desc())
+    n = _native.lib().fstx_orthogonalize_workspace(arr, 1, c, 1)
+    assert n > 0
     for args in ((arr, 1, c, 0, 0.0, 0x1000, n), (arr, 1, c, 65, 0.0, 0x1000, n), (arr, 1, None, 1, 0.0, 0x1000, n),
                  (arr, 1, c, 1, -1.0, 0x1000, n), (arr, 1, c, 1, float("nan"), 0x1000, n), (arr, 1, c, 1, 0.0, None, n),
                  (arr, 1, c, 1, 0.0, 0x1010, n), (arr, 1, c, 1, 0.0, 0x1000, n - 1), (None, 1, c, 1, 0.0, 0x1000, n)):
