@@ -10,9 +10,18 @@
 //                        against M N of the weight, and are re-read by every tile they feed, so that
 //                        strides, element types, odd sizes and zero padding are dealt with once
 //                        and the main kernel has none of them.
-//   low_rank_kernel      one wavefront per 64 x 64 tile of W: loads its tile of W first (all of it
-//                        in flight), accumulates the product from operands that L2 holds, adds,
-//                        rounds, stores.  No LDS and no barriers: nothing is shared but the factors.
+//   low_rank_kernel      a wavefront walks along a panel of rows in tiles of one 128-byte line per row (64 rows;
+//                        32 of fp8): the next tile's weights are on their way while it makes the product
+//                        of this one from operands that L2 holds, adds, rounds and stores.
+//                        No LDS and no barriers: nothing is shared but the factors.
+//
+// What bounds it, measured.  The seven matrices of a Llama-3-8B layer, bf16, rank 64 (883 MB read and written):
+// 169 us + 15 us of packing, 5.2 TB/s; a plain copy of that size does 6.2.  A Llama-3-70B fp8 layer, rank 16
+// (1.7 GB): 360 us, 4.8 TB/s.  Steps there (same layer): one 64 x 64 tile per wavefront with 64 contiguous bytes per row and
+// instruction 241 us, 26 % more written to HBM than the weight holds, because half lines left L2 before their other
+// halves came; whole lines per instruction 193 us; walks of four tiles 184 (of eight 189, of two 180 but 364 instead of
+// 359 for the fp8 layer).  Streaming (non-temporal) accesses are worth 5 to 8 % where rows lie on whole lines and cost 25 %
+// where tiles share them: see on_lines.
 //
 // Numerics.  MFMA products of bf16 / fp16 are exact in fp32 and are summed in fp32.  Factors of
 // f32 are split into bf16 terms x = h + m (+ l), each the rounding of what is left: bf16 because it
@@ -26,9 +35,9 @@
 // lane order, 1 KiB, so that an operand load is one fully coalesced global_load_dwordx4.  The
 // product is computed transposed (D as the first operand): a lane then holds, for ONE row of W, the
 // 4 columns that its quarter of the wavefront owns in each 16-column block; and the columns are
-// dealt to the blocks so that the blocks of one 16-byte vector of W are consecutive (column_of):
-// W goes straight between memory and the accumulator layout, 16 bytes per lane, 64 contiguous
-// bytes per row and instruction.
+// dealt to the blocks so that the blocks of one 16-byte vector of W are consecutive (column_of).
+// Two lanes of neighbouring rows trade their halves of the two lines (trade), and W moves
+// between memory and the accumulator layout 16 bytes per lane and a whole line per row and instruction.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -45,10 +54,10 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
-constexpr uint32_t kTile = 64;   // rows and columns of W per wavefront
+constexpr uint32_t kTile = 128;  // rows and columns the packed factors are padded to: whole tiles of every type
 constexpr uint32_t kBlk = 512;   // elements of one operand block (16 rows x 32 k)
 constexpr uint32_t kK = 32;      // k per block
-constexpr uint32_t kMaxJobs = 32;
+constexpr uint32_t kMaxJobs = 24;
 
 // How the factors travel: the type and number of their terms.
 enum : uint32_t { kTermsH1 = 0, kTermsB1 = 1, kTermsB2 = 2, kTermsB3 = 3, kTermClasses = 4 };
@@ -62,10 +71,12 @@ struct alignas(32) MergeJob {
     uint64_t dst_pitch, src_pitch; // bytes
     uint32_t rows, cols, k_blocks, col_tiles;
     float scale;
-    uint32_t scale_step; // 0: one weight scale, 1: one per row
-    uint32_t n_tiles, pad;
+    uint32_t scale_step;           // 0: one weight scale, 1: one per row
+    uint32_t walk, walks, n_walks; // tiles per wavefront, wavefronts per panel of rows and in all
+    uint32_t lines;                // see on_lines
+    uint32_t pad[2];
 };
-static_assert(sizeof(MergeJob) == 96, "32 of them fit the kernel arguments");
+static_assert(sizeof(MergeJob) == 128, "24 of them fit the kernel arguments");
 
 struct PackJob {
     const char *src;
@@ -108,13 +119,13 @@ __device__ __forceinline__ float bf16_term(float x) {
     return h;
 }
 
-// One wavefront per operand block.
-__global__ __launch_bounds__(64) void pack_factors_kernel(const Jobs<PackJob> t) {
+// One wavefront per operand block, four per workgroup (a side has a multiple of eight blocks).
+__global__ __launch_bounds__(256) void pack_factors_kernel(const Jobs<PackJob> t) {
     const uint32_t ji = job_of(t, blockIdx.x);
     const PackJob &job = t.job[ji];
-    const uint32_t lb = blockIdx.x - t.first[ji];
+    const uint32_t lb = (blockIdx.x - t.first[ji]) * 4 + (threadIdx.x >> 6);
     const uint32_t blk = lb / job.k_blocks, kb = lb - blk * job.k_blocks;
-    const uint32_t lane = threadIdx.x, rho = lane & 15;
+    const uint32_t lane = threadIdx.x & 63, rho = lane & 15;
     const uint32_t row = job.per ? column_of(blk, rho, job.per) : blk * 16 + rho;
     const uint32_t k0 = kb * kK + 8 * (lane >> 4);
     float x[8];
@@ -201,110 +212,229 @@ __device__ __forceinline__ v4u merged(v4u w, const float *acc, float s) {
     return out;
 }
 
-template <uint32_t T, uint32_t Cls, bool Edge>
-__device__ __forceinline__ void merge_tile(const MergeJob &job, uint32_t r0, uint32_t c0) {
+// Lanes 2n and 2n + 1 (two rows of a tile): what the even one holds in b against what the odd one holds in a.
+// Each row's two halves of a line, held by one lane each way, become two whole lines held by both: its own inverse.
+__device__ __forceinline__ void trade(v4u &a, v4u &b, bool odd) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t give = odd ? a[k] : b[k];
+        const uint32_t got = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)give, 0xb1 /* quad_perm:[1,0,3,2] */, 0xf, 0xf, true);
+        const uint32_t x = odd ? got : a[k], y = odd ? b[k] : got;
+        a[k] = x;
+        b[k] = y;
+    }
+}
+
+// Shape of a wavefront's tile: kRows rows of one 128-byte line.
+template <uint32_t T> struct Tile {
+    static constexpr uint32_t kSize = Weight<T>::size, kPer = 16 / kSize;
+    static constexpr uint32_t kCols = 128 / kSize;                // 32, 64 or 128
+    static constexpr uint32_t kRows = kSize == 1 ? 32 : 64;
+    static constexpr uint32_t kNR = kRows / 16, kNC = kCols / 16; // operand blocks
+};
+
+// The 1..15 bytes that end a row, in pieces of 8, 4, 2 and 1: all loads of a wavefront at once, where a loop over
+// elements would wait for each.
+__device__ __forceinline__ v4u load_tail(const char *at, uint32_t bytes) {
+    typedef uint64_t by1_8 __attribute__((aligned(1)));
+    typedef uint32_t by1_4 __attribute__((aligned(1)));
+    typedef uint16_t by1_2 __attribute__((aligned(1)));
+    unsigned __int128 v = 0;
+    if (bytes & 8) v = *(const FSTX_GLOBAL by1_8 *)at;
+    if (bytes & 4) v |= (unsigned __int128) * (const FSTX_GLOBAL by1_4 *)(at + (bytes & 8)) << 8 * (bytes & 8);
+    if (bytes & 2) v |= (unsigned __int128) * (const FSTX_GLOBAL by1_2 *)(at + (bytes & 12)) << 8 * (bytes & 12);
+    if (bytes & 1) v |= (unsigned __int128) * (const FSTX_GLOBAL uint8_t *)(at + (bytes & 14)) << 8 * (bytes & 14);
+    return __builtin_bit_cast(v4u, v);
+}
+__device__ __forceinline__ void store_tail(char *at, uint32_t bytes, v4u value) {
+    typedef uint64_t by1_8 __attribute__((aligned(1)));
+    typedef uint32_t by1_4 __attribute__((aligned(1)));
+    typedef uint16_t by1_2 __attribute__((aligned(1)));
+    const unsigned __int128 v = __builtin_bit_cast(unsigned __int128, value);
+    if (bytes & 8) *(FSTX_GLOBAL by1_8 *)at = (uint64_t)v;
+    if (bytes & 4) *(FSTX_GLOBAL by1_4 *)(at + (bytes & 8)) = (uint32_t)(v >> 8 * (bytes & 8));
+    if (bytes & 2) *(FSTX_GLOBAL by1_2 *)(at + (bytes & 12)) = (uint16_t)(v >> 8 * (bytes & 12));
+    if (bytes & 1) *(FSTX_GLOBAL uint8_t *)(at + (bytes & 14)) = (uint8_t)(v >> 8 * (bytes & 14));
+}
+
+template <uint32_t T, uint32_t Cls, uint32_t NR = Tile<T>::kNR> struct Merge {
+    typedef Tile<T> S;
     typedef typename Operand<Cls>::type op_t;
     typedef typename Weight<T>::loose loose_t;
-    constexpr uint32_t kTerms = terms_of(Cls), kSize = Weight<T>::size, kPer = 16 / kSize;
-    constexpr uint32_t kVecs = kTile / (4 * kPer); // 16-byte vectors per lane and row
-    constexpr uint32_t kNB = kTile / 16;           // operand blocks along either side
-    const uint32_t lane = threadIdx.x, g = lane >> 4;
+    static constexpr uint32_t kTerms = terms_of(Cls), kNR = NR, kNC = S::kNC, kPer = S::kPer;
 
-    // the tile of W, all of it in flight before the product begins
-    v4u w[kNB][kVecs];
+    // the tile's vectors: [i][0] and [i][1] are the two halves of the line of row 16 i + lane % 16
+    // Whole lines, which only this wavefront touches, are streamed past L2 (Stream); where tiles share lines they meet there.
+    template <bool Edge, bool Stream> static __device__ __forceinline__ void load(const MergeJob &job, uint32_t r0, uint32_t c0, uint32_t lane, v4u (&w)[kNR][2]) {
+        const uint32_t col = c0 + (lane & 1) * 4 * kPer + (lane >> 4) * kPer;
 #pragma unroll
-    for (uint32_t i = 0; i < kNB; ++i) {
-        const uint32_t row = r0 + 16 * i + (lane & 15);
-        const char *at = job.src + (uint64_t)row * job.src_pitch;
+        for (uint32_t i = 0; i < kNR; ++i)
 #pragma unroll
-        for (uint32_t v = 0; v < kVecs; ++v) {
-            const uint32_t col = c0 + v * 4 * kPer + g * kPer;
-            if (!Edge || (row < job.rows && col + kPer <= job.cols)) {
-                w[i][v] = __builtin_nontemporal_load((const FSTX_GLOBAL loose_t *)(at + (uint64_t)col * kSize));
-            } else {
-                w[i][v] = v4u{0, 0, 0, 0};
-                if (row < job.rows && col < job.cols) { // the vector that ends the row: element by element
-                    uint8_t part[16] = {};
-                    for (uint32_t e = 0; e < (job.cols - col) * kSize; ++e) part[e] = *(const FSTX_GLOBAL uint8_t *)(at + (uint64_t)col * kSize + e);
-                    __builtin_memcpy(&w[i][v], part, 16);
+            for (uint32_t v = 0; v < 2; ++v) { // as loaded: even rows, then odd rows, a line by eight lanes
+                const uint32_t row = r0 + 16 * i + (lane & 14) + v;
+                const char *at = job.src + (uint64_t)row * job.src_pitch + (uint64_t)col * S::kSize;
+                if (!Edge || (row < job.rows && col + kPer <= job.cols)) {
+                    if constexpr (Stream) w[i][v] = __builtin_nontemporal_load((const FSTX_GLOBAL loose_t *)at);
+                    else w[i][v] = *(const FSTX_GLOBAL loose_t *)at;
+                } else {
+                    w[i][v] = v4u{0, 0, 0, 0};
+                    if (row < job.rows && col < job.cols) w[i][v] = load_tail(at, (job.cols - col) * S::kSize);
+                }
+            }
+    }
+
+    template <bool Edge, bool Stream>
+    static __device__ __forceinline__ void finish(const MergeJob &job, uint32_t r0, uint32_t c0, uint32_t lane, v4u (&w)[kNR][2], const v4f (&acc)[kNR][kNC],
+                                                  const float (&scale)[kNR]) {
+        const uint32_t col = c0 + (lane & 1) * 4 * kPer + (lane >> 4) * kPer;
+#pragma unroll
+        for (uint32_t i = 0; i < kNR; ++i) {
+            trade(w[i][0], w[i][1], lane & 1);
+#pragma unroll
+            for (uint32_t v = 0; v < 2; ++v) {
+                float sums[kPer];
+#pragma unroll
+                for (uint32_t e = 0; e < kPer; ++e) sums[e] = acc[i][v * (kPer / 4) + e / 4][e % 4];
+                w[i][v] = merged<T>(w[i][v], sums, scale[i]);
+            }
+            trade(w[i][0], w[i][1], lane & 1);
+#pragma unroll
+            for (uint32_t v = 0; v < 2; ++v) {
+                const uint32_t row = r0 + 16 * i + (lane & 14) + v;
+                char *at = job.dst + (uint64_t)row * job.dst_pitch + (uint64_t)col * S::kSize;
+                if (!Edge || (row < job.rows && col + kPer <= job.cols)) {
+                    if constexpr (Stream) __builtin_nontemporal_store(w[i][v], (FSTX_GLOBAL loose_t *)at);
+                    else *(FSTX_GLOBAL loose_t *)at = w[i][v];
+                } else if (row < job.rows && col < job.cols) {
+                    store_tail(at, (job.cols - col) * S::kSize, w[i][v]);
                 }
             }
         }
     }
-    float row_scale[kNB];
+
+    static __device__ __forceinline__ void fetch(const uint16_t *at, uint64_t step, op_t (&f)[kTerms], uint32_t i) {
 #pragma unroll
-    for (uint32_t i = 0; i < kNB; ++i) {
-        row_scale[i] = job.scale;
-        if constexpr (T == FSTX_F8_E4M3) {
-            const uint32_t row = r0 + 16 * i + (lane & 15);
-            const uint32_t at = Edge && row >= job.rows ? 0 : row;
-            row_scale[i] = job.scale / *(const FSTX_GLOBAL float *)(job.weight_scale + (uint64_t)at * job.scale_step);
-        }
+        for (uint32_t p = 0; p < kTerms; ++p) f[p] = *(const FSTX_GLOBAL op_t *)(at + i * step + p * kBlk);
     }
 
-    v4f acc[kNB][kNB] = {};
-    const uint16_t *up = job.up + (uint64_t)(r0 / 16) * job.k_blocks * kTerms * kBlk + lane * 8;
-    const uint16_t *down = job.down + (uint64_t)(c0 / 16) * job.k_blocks * kTerms * kBlk + lane * 8;
-    const uint64_t step = (uint64_t)job.k_blocks * kTerms * kBlk;
-    for (uint32_t kb = 0; kb < job.k_blocks; ++kb) {
-        op_t u[kNB][kTerms], d[kNB][kTerms];
+    // term a of one factor with term b of the other as long as a + b < terms, small ones first
+    static __device__ __forceinline__ void multiply(const op_t (&u)[kNR][kTerms], const op_t (&d)[kNC][kTerms], v4f (&acc)[kNR][kNC]) {
 #pragma unroll
-        for (uint32_t i = 0; i < kNB; ++i)
+        for (int sum = (int)kTerms - 1; sum >= 0; --sum)
 #pragma unroll
-            for (uint32_t p = 0; p < kTerms; ++p) {
-                u[i][p] = *(const FSTX_GLOBAL op_t *)(up + i * step + p * kBlk);
-                d[i][p] = *(const FSTX_GLOBAL op_t *)(down + i * step + p * kBlk);
-            }
+            for (int a = 0; a <= sum; ++a)
 #pragma unroll
-        for (uint32_t i = 0; i < kNB; ++i)
+                for (uint32_t i = 0; i < kNR; ++i)
 #pragma unroll
-            for (uint32_t j = 0; j < kNB; ++j)
-                // term a of one factor with term b of the other as long as a + b < terms, small ones first
-#pragma unroll
-                for (int sum = (int)kTerms - 1; sum >= 0; --sum)
-#pragma unroll
-                    for (int a = 0; a <= sum; ++a) acc[i][j] = mfma(d[j][a], u[i][sum - a], acc[i][j]);
-        up += kTerms * kBlk;
-        down += kTerms * kBlk;
+                    for (uint32_t j = 0; j < kNC; ++j) acc[i][j] = mfma(d[j][a], u[i][sum - a], acc[i][j]);
     }
 
+    // one tile whose weights are in w (or on their way)
+    template <uint32_t kHeld, bool Edge, bool Stream>
+    static __device__ __forceinline__ void tile(const MergeJob &job, uint32_t r0, uint32_t c0, uint32_t lane, v4u (&w)[kNR][2],
+                                                const op_t (&held)[kHeld ? kHeld : 1][kNR][kTerms], const op_t (&d)[kHeld ? kHeld : 1][kNC][kTerms],
+                                                const float (&scale)[kNR]) {
+        v4f acc[kNR][kNC] = {};
+        if constexpr (kHeld > 0) {
 #pragma unroll
-    for (uint32_t i = 0; i < kNB; ++i) {
-        const uint32_t row = r0 + 16 * i + (lane & 15);
-        char *at = job.dst + (uint64_t)row * job.dst_pitch;
+            for (uint32_t kb = 0; kb < kHeld; ++kb) multiply(held[kb], d[kb], acc);
+        } else {
+            const uint64_t step = (uint64_t)job.k_blocks * kTerms * kBlk;
+            const uint16_t *up = job.up + r0 / 16 * step + lane * 8, *down = job.down + c0 / 16 * step + lane * 8;
+            for (uint32_t kb = 0; kb < job.k_blocks; ++kb, up += kTerms * kBlk, down += kTerms * kBlk) {
+                op_t u[kNR][kTerms], dd[kNC][kTerms];
 #pragma unroll
-        for (uint32_t v = 0; v < kVecs; ++v) {
-            const uint32_t col = c0 + v * 4 * kPer + g * kPer;
-            float sums[kPer];
+                for (uint32_t i = 0; i < kNR; ++i) fetch(up, step, u[i], i);
 #pragma unroll
-            for (uint32_t e = 0; e < kPer; ++e) sums[e] = acc[i][v * (kPer / 4) + e / 4][e % 4];
-            const v4u out = merged<T>(w[i][v], sums, row_scale[i]);
-            if (!Edge || (row < job.rows && col + kPer <= job.cols)) {
-                __builtin_nontemporal_store(out, (FSTX_GLOBAL loose_t *)(at + (uint64_t)col * kSize));
-            } else if (row < job.rows && col < job.cols) {
-                uint8_t part[16];
-                __builtin_memcpy(part, &out, 16);
-                for (uint32_t e = 0; e < (job.cols - col) * kSize; ++e) *(FSTX_GLOBAL uint8_t *)(at + (uint64_t)col * kSize + e) = part[e];
+                for (uint32_t j = 0; j < kNC; ++j) fetch(down, step, dd[j], j);
+                multiply(u, dd, acc);
             }
         }
+        finish<Edge, Stream>(job, r0, c0, lane, w, acc, scale);
     }
-}
 
-template <uint32_t T, uint32_t Cls>
-__global__ __launch_bounds__(64) void low_rank_kernel(const uint32_t dies_log2, const Jobs<MergeJob> t) {
+    // A wavefront walks along a panel of kRows rows: the rows' factor stays in registers (kHeld blocks of 32 k; 0: too
+    // many, both factors are read per tile), the columns' factor comes from L2, and the weights of the next tile are on
+    // their way while one is worked on.
+    // (Stream and the tiles at the edges are told apart outside the loop: with a branch around the loads the compiler
+    // would have to wait for all of them.)
+    template <uint32_t kHeld, bool Stream> static __device__ __forceinline__ void walk(const MergeJob &job, uint32_t r0, uint32_t first, uint32_t last, uint32_t lane) {
+        constexpr uint32_t kH = kHeld ? kHeld : 1;
+        float scale[kNR];
+#pragma unroll
+        for (uint32_t i = 0; i < kNR; ++i) {
+            scale[i] = job.scale;
+            if constexpr (T == FSTX_F8_E4M3) {
+                const uint32_t row = r0 + 16 * i + (lane & 15), at = row < job.rows ? row : 0;
+                scale[i] = job.scale / *(const FSTX_GLOBAL float *)(job.weight_scale + (uint64_t)at * job.scale_step);
+            }
+        }
+        const uint64_t step = (uint64_t)job.k_blocks * kTerms * kBlk;
+        op_t held[kH][kNR][kTerms], d[kH][kNC][kTerms];
+        if constexpr (kHeld > 0)
+#pragma unroll
+            for (uint32_t kb = 0; kb < kHeld; ++kb)
+#pragma unroll
+                for (uint32_t i = 0; i < kNR; ++i) fetch(job.up + r0 / 16 * step + kb * kTerms * kBlk + lane * 8, step, held[kb][i], i);
+        auto columns = [&](uint32_t t) {
+            if constexpr (kHeld > 0)
+#pragma unroll
+                for (uint32_t kb = 0; kb < kHeld; ++kb)
+#pragma unroll
+                    for (uint32_t j = 0; j < kNC; ++j) fetch(job.down + (uint64_t)t * kNC * step + kb * kTerms * kBlk + lane * 8, step, d[kb][j], j);
+        };
+        const uint32_t whole = r0 + 16 * kNR <= job.rows ? job.cols / S::kCols : 0; // tiles of the panel without an edge
+        const uint32_t full = last < whole ? last : whole;
+        v4u w[kNR][2], next[kNR][2];
+        auto advance = [&]() {
+#pragma unroll
+            for (uint32_t i = 0; i < kNR; ++i)
+#pragma unroll
+                for (uint32_t v = 0; v < 2; ++v) w[i][v] = next[i][v];
+        };
+        uint32_t t = first;
+        if (t < full) {
+            load<false, Stream>(job, r0, t * S::kCols, lane, w);
+            for (; t + 1 < full; ++t) {
+                columns(t);
+                load<false, Stream>(job, r0, (t + 1) * S::kCols, lane, next);
+                tile<kHeld, false, Stream>(job, r0, t * S::kCols, lane, w, held, d, scale);
+                advance();
+            }
+            columns(t);
+            if (t + 1 < last) load<true, false>(job, r0, (t + 1) * S::kCols, lane, next);
+            tile<kHeld, false, Stream>(job, r0, t * S::kCols, lane, w, held, d, scale);
+            advance();
+            ++t;
+        } else {
+            load<true, false>(job, r0, t * S::kCols, lane, w);
+        }
+        for (; t < last; ++t) {
+            columns(t);
+            if (t + 1 < last) load<true, false>(job, r0, (t + 1) * S::kCols, lane, next);
+            tile<kHeld, true, false>(job, r0, t * S::kCols, lane, w, held, d, scale);
+            advance();
+        }
+    }
+};
+
+template <uint32_t T, uint32_t Cls, uint32_t kHeld>
+__global__ __launch_bounds__(64, 2) void low_rank_kernel(const uint32_t dies_log2, const Jobs<MergeJob> t) {
     const uint32_t ji = job_of(t, blockIdx.x);
     const MergeJob &job = t.job[ji];
-    uint32_t tile;
-    if (!fstx_gather::tile_for_die(blockIdx.x - t.first[ji], job.n_tiles, dies_log2, tile)) return;
-    const uint32_t rt = tile / job.col_tiles, ct = tile - rt * job.col_tiles;
-    const uint32_t r0 = rt * kTile, c0 = ct * kTile;
-    if (r0 + kTile <= job.rows && c0 + kTile <= job.cols) merge_tile<T, Cls, false>(job, r0, c0);
-    else merge_tile<T, Cls, true>(job, r0, c0);
+    uint32_t at;
+    if (!fstx_gather::tile_for_die(blockIdx.x - t.first[ji], job.n_walks, dies_log2, at)) return;
+    const uint32_t panel = at / job.walks, nth = at - panel * job.walks; // neighbours walk along the same panel
+    const uint32_t first = nth * job.walk, last = first + job.walk < job.col_tiles ? first + job.walk : job.col_tiles;
+    if (job.lines == 3) Merge<T, Cls>::template walk<kHeld, true>(job, panel * Tile<T>::kRows, first, last, threadIdx.x);
+    else Merge<T, Cls>::template walk<kHeld, false>(job, panel * Tile<T>::kRows, first, last, threadIdx.x);
 }
 
 // --------------------------------------------------------------- host side
 
 constexpr uint64_t kMaxSide = 0x7fffff00ull;    // rows, columns: positions stay in 32 bits
+constexpr uint64_t kWaves = 4096;          // wavefronts that fill the device (eight per compute unit) twice
+constexpr uint64_t kLongestWalk = 4;
 constexpr uint64_t kLaunchBlocks = 48ull << 20; // workgroups of 64 lanes per launch: 32 bits of lanes
 
 inline uint32_t size_of(uint32_t type) { return type == FSTX_F32 ? 4 : type == FSTX_F8_E4M3 ? 1 : 2; }
@@ -365,7 +495,7 @@ int check(const fstx_low_rank_desc *descs, uint32_t n) {
         if (eight ? !d.weight_scale || (uintptr_t)d.weight_scale % 4 || (d.n_weight_scales != 1 && d.n_weight_scales != d.rows)
                   : d.weight_scale != nullptr || d.n_weight_scales != 0)
             return -FSTX_E_INVAL;
-        const uint64_t tiles = (d.rows + kTile - 1) / kTile * ((d.cols + kTile - 1) / kTile);
+        const uint64_t tiles = (d.rows + 31) / 32 * ((d.cols + 31) / 32); // more than there are of any type
         if (tiles > kLaunchBlocks / 2 || (blocks16(d.rows) + blocks16(d.cols)) * k_blocks_of(d) > kLaunchBlocks / 2) return -FSTX_E_RANGE;
         // in place, or a source that the destination does not touch
         const bool in_place = d.dst == d.src && (d.rows == 1 || d.dst_pitch == d.src_pitch);
@@ -394,12 +524,18 @@ template <typename Job> void clear(Jobs<Job> &t) {
     for (uint32_t i = 0; i < kMaxJobs; ++i) t.first[i] = 0xffffffffu;
 }
 
-template <uint32_t T, uint32_t Cls> void launch(uint32_t grid, const Jobs<MergeJob> &t, hipStream_t s) {
-    hipLaunchKernelGGL((low_rank_kernel<T, Cls>), dim3(grid), dim3(64), 0, s, fstx_internal::dies_log2(), t);
+// Blocks of 32 k of the rows' factor that stay in registers
+template <uint32_t T, uint32_t Cls> constexpr uint32_t held_most() { return Cls == kTermsB3 ? 1 : Cls == kTermsB2 ? 1 : 2; }
+
+template <uint32_t T, uint32_t Cls> void launch(uint32_t grid, uint32_t held, const Jobs<MergeJob> &t, hipStream_t s) {
+    const uint32_t dies = fstx_internal::dies_log2();
+    if (held == 1) hipLaunchKernelGGL((low_rank_kernel<T, Cls, 1>), dim3(grid), dim3(64), 0, s, dies, t);
+    else if (held == 2 && held_most<T, Cls>() >= 2) hipLaunchKernelGGL((low_rank_kernel<T, Cls, held_most<T, Cls>() >= 2 ? 2 : 1>), dim3(grid), dim3(64), 0, s, dies, t);
+    else hipLaunchKernelGGL((low_rank_kernel<T, Cls, 0>), dim3(grid), dim3(64), 0, s, dies, t);
 }
 
-void launch_class(uint32_t type, uint32_t cls, uint32_t grid, const Jobs<MergeJob> &t, hipStream_t s) {
-#define FSTX_CASE(T, C) case (T) * kTermClasses + (C): launch<T, C>(grid, t, s); break;
+void launch_class(uint32_t type, uint32_t cls, uint32_t held, uint32_t grid, const Jobs<MergeJob> &t, hipStream_t s) {
+#define FSTX_CASE(T, C) case (T) * kTermClasses + (C): launch<T, C>(grid, held, t, s); break;
     switch (type * kTermClasses + cls) {
         FSTX_CASE(FSTX_F32, kTermsH1) FSTX_CASE(FSTX_F32, kTermsB1) FSTX_CASE(FSTX_F32, kTermsB3)
         FSTX_CASE(FSTX_BF16, kTermsH1) FSTX_CASE(FSTX_BF16, kTermsB1) FSTX_CASE(FSTX_BF16, kTermsB2)
@@ -408,6 +544,18 @@ void launch_class(uint32_t type, uint32_t cls, uint32_t grid, const Jobs<MergeJo
     default: break; // class_of gives no others
     }
 #undef FSTX_CASE
+}
+
+// whether rows lie on whole 128-byte lines: bit 0 the destination's, bit 1 the source's
+inline uint32_t on_lines(const fstx_low_rank_desc &d) {
+    const uint64_t size = size_of(d.type), dp = d.rows == 1 ? 0 : d.dst_pitch * size, sp = d.rows == 1 ? 0 : d.src_pitch * size;
+    return ((((uint64_t)(uintptr_t)d.dst | dp) & 127) == 0 ? 1u : 0u) | ((((uint64_t)(uintptr_t)d.src | sp) & 127) == 0 ? 2u : 0u);
+}
+
+// which kernel variant serves a descriptor
+inline uint32_t held_of(const fstx_low_rank_desc &d) {
+    const uint64_t kb = k_blocks_of(d), most = terms_of(class_of(d)) > 1 ? 1 : 2;
+    return kb == 0 ? 0 : kb <= most ? (uint32_t)kb : 0;
 }
 
 } // namespace
@@ -435,7 +583,7 @@ extern "C" int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, 
         auto flush = [&]() -> int {
             if (k == 0) return 0;
             fstx_internal::Range range("fstx pack_factors_kernel: %u jobs, %llu workgroups", k, (unsigned long long)grid);
-            hipLaunchKernelGGL(pack_factors_kernel, dim3((uint32_t)grid), dim3(64), 0, s, t);
+            hipLaunchKernelGGL(pack_factors_kernel, dim3((uint32_t)grid), dim3(256), 0, s, t);
             k = 0;
             grid = 0;
             clear(t);
@@ -444,7 +592,7 @@ extern "C" int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, 
         for (uint32_t i = 0; i < n; ++i) {
             const fstx_low_rank_desc &d = descs[i];
             if (empty(d) || d.rank == 0) continue;
-            const uint64_t kb = k_blocks_of(d), need_blocks = (blocks16(d.rows) + blocks16(d.cols)) * kb;
+            const uint64_t kb = k_blocks_of(d), need_blocks = (blocks16(d.rows) + blocks16(d.cols)) * kb / 4;
             if (k + 2 > kMaxJobs || grid + need_blocks > kLaunchBlocks) {
                 const int rc = flush();
                 if (rc < 0) return rc;
@@ -457,7 +605,7 @@ extern "C" int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, 
                                 : PackJob{static_cast<const char *>(d.up), space + at, d.up_row_stride, d.up_col_stride, (uint32_t)len,
                                           (uint32_t)d.rank, (uint32_t)kb, (uint32_t)blocks16(len), d.up_type, terms_of(cls), cls == kTermsH1, 0};
                 t.first[k++] = (uint32_t)grid;
-                grid += blocks16(len) * kb;
+                grid += blocks16(len) * kb / 4;
                 at += packed_elems(len, d);
             }
         }
@@ -467,42 +615,48 @@ extern "C" int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, 
     // one launch (or a few) per kernel variant that occurs
     static const uint32_t types[4] = {FSTX_F32, FSTX_BF16, FSTX_F16, FSTX_F8_E4M3};
     const uint64_t dies = 1ull << fstx_internal::dies_log2();
-    for (uint32_t type : types)
-        for (uint32_t cls = 0; cls < kTermClasses; ++cls) {
-            Jobs<MergeJob> t;
+    for (uint32_t variant = 0; variant < 4 * kTermClasses * 3; ++variant) {
+        const uint32_t type = types[variant / (kTermClasses * 3)], cls = variant / 3 % kTermClasses, held = variant % 3;
+        Jobs<MergeJob> t;
+        clear(t);
+        uint32_t k = 0;
+        uint64_t grid = 0, at = 0;
+        auto flush = [&]() -> int {
+            if (k == 0) return 0;
+            fstx_internal::Range range("fstx low_rank_kernel: %u jobs, %llu workgroups", k, (unsigned long long)grid);
+            launch_class(type, cls, held, (uint32_t)grid, t, s);
+            k = 0;
+            grid = 0;
             clear(t);
-            uint32_t k = 0;
-            uint64_t grid = 0, at = 0;
-            auto flush = [&]() -> int {
-                if (k == 0) return 0;
-                fstx_internal::Range range("fstx low_rank_kernel: %u jobs, %llu workgroups", k, (unsigned long long)grid);
-                launch_class(type, cls, (uint32_t)grid, t, s);
-                k = 0;
-                grid = 0;
-                clear(t);
-                return fstx_internal::check_launch("low_rank_kernel");
-            };
-            for (uint32_t i = 0; i < n; ++i) {
-                const fstx_low_rank_desc &d = descs[i];
-                if (empty(d)) continue;
-                const uint64_t up_at = at, down_at = at + packed_elems(d.rows, d);
-                at = down_at + packed_elems(d.cols, d);
-                if (d.type != type || class_of(d) != cls) continue;
-                const uint64_t col_tiles = (d.cols + kTile - 1) / kTile, tiles = (d.rows + kTile - 1) / kTile * col_tiles;
-                const uint64_t blocks = (tiles + dies - 1) / dies * dies;
-                if (k == kMaxJobs || grid + blocks > kLaunchBlocks) {
-                    const int rc = flush();
-                    if (rc < 0) return rc;
-                }
-                const uint64_t size = size_of(type);
-                t.job[k] = MergeJob{static_cast<char *>(d.dst), static_cast<const char *>(d.src), space + up_at, space + down_at, d.weight_scale,
-                                    d.dst_pitch * size, d.src_pitch * size, (uint32_t)d.rows, (uint32_t)d.cols, (uint32_t)k_blocks_of(d),
-                                    (uint32_t)col_tiles, d.scale, d.n_weight_scales > 1 ? 1u : 0u, (uint32_t)tiles, 0};
-                t.first[k++] = (uint32_t)grid;
-                grid += blocks;
+            return fstx_internal::check_launch("low_rank_kernel");
+        };
+        const uint64_t size = size_of(type), tile_cols = 128 / size, tile_rows = size == 1 ? 32 : 64;
+        uint64_t tiles = 0; // of the whole call, for the length of the walks
+        for (uint32_t i = 0; i < n; ++i)
+            if (!empty(descs[i])) tiles += (descs[i].cols + tile_cols - 1) / tile_cols * ((descs[i].rows + tile_rows - 1) / tile_rows);
+        for (uint32_t i = 0; i < n; ++i) {
+            const fstx_low_rank_desc &d = descs[i];
+            if (empty(d)) continue;
+            const uint64_t up_at = at, down_at = at + packed_elems(d.rows, d);
+            at = down_at + packed_elems(d.cols, d);
+            if (d.type != type || class_of(d) != cls || held_of(d) != held) continue;
+            const uint64_t col_tiles = (d.cols + tile_cols - 1) / tile_cols, panels = (d.rows + tile_rows - 1) / tile_rows;
+            uint64_t walk = tiles / kWaves;
+            walk = walk < 1 ? 1 : walk > kLongestWalk ? kLongestWalk : walk;
+            const uint64_t walks = (col_tiles + walk - 1) / walk;
+            const uint64_t blocks = (panels * walks + dies - 1) / dies * dies;
+            if (k == kMaxJobs || grid + blocks > kLaunchBlocks) {
+                const int rc = flush();
+                if (rc < 0) return rc;
             }
-            const int rc = flush();
-            if (rc < 0) return rc;
+            t.job[k] = MergeJob{static_cast<char *>(d.dst), static_cast<const char *>(d.src), space + up_at, space + down_at, d.weight_scale,
+                                d.dst_pitch * size, d.src_pitch * size, (uint32_t)d.rows, (uint32_t)d.cols, (uint32_t)k_blocks_of(d),
+                                (uint32_t)col_tiles, d.scale, d.n_weight_scales > 1 ? 1u : 0u, (uint32_t)walk, (uint32_t)walks, (uint32_t)(panels * walks), on_lines(d), {}};
+            t.first[k++] = (uint32_t)grid;
+            grid += blocks;
         }
+        const int rc = flush();
+        if (rc < 0) return rc;
+    }
     return 0;
 }

@@ -40,12 +40,12 @@ def test_header_and_binding_list_the_same_functions_and_layouts(tmp_path):
 def test_workspace_sizes():
     assert need() == 0
     assert need(desc(rows=0)) == need(desc(cols=0)) == need(desc(rank=0, up=None, down=None)) == 0
-    # 100 x 60 at rank 8: (128 + 64) rows of 32 k, 2 bytes, one term
-    assert need(desc()) == 192 * 32 * 2
-    assert need(desc(ftype=F32)) == 2 * 192 * 32 * 2
-    assert need(desc(ftype=F32, type=F32)) == 3 * 192 * 32 * 2
-    assert need(desc(rank=33)) == 192 * 64 * 2
-    assert need(desc(), desc(dst=0x2000000)) == 2 * 192 * 32 * 2
+    # 100 x 60 at rank 8: (128 + 128) rows of 32 k, 2 bytes, one term
+    assert need(desc()) == 256 * 32 * 2
+    assert need(desc(ftype=F32)) == 2 * 256 * 32 * 2
+    assert need(desc(ftype=F32, type=F32)) == 3 * 256 * 32 * 2
+    assert need(desc(rank=33)) == 256 * 64 * 2
+    assert need(desc(), desc(dst=0x2000000)) == 2 * 256 * 32 * 2
 
 
 @pytest.mark.parametrize("bad", [
