@@ -10,6 +10,7 @@
 //                        against M N of the weight, and are re-read by every tile they feed, so that
 //                        strides, element types, odd sizes and zero padding are dealt with once
 //                        and the main kernel has none of them.
+//   deep_low_rank_kernel for longer products, direct_low_rank_kernel for few tiles: see there.
 //   low_rank_kernel      a wavefront walks along a panel of rows in tiles of one 128-byte line per row (64 rows;
 //                        32 of fp8): the next tile's weights are on their way while it makes the product
 //                        of this one from operands that L2 holds, adds, rounds and stores.
@@ -26,8 +27,8 @@
 // Numerics.  MFMA products of bf16 / fp16 are exact in fp32 and are summed in fp32.  Factors of
 // f32 are split into bf16 terms x = h + m (+ l), each the rounding of what is left: bf16 because it
 // has f32's range.  Two terms (16 bits of each factor; h h + h m + m h, what is left out is below
-// 2^-17 of a product) for weights of 8 or 16 bits, whose own rounding is 2^-12 at best; three terms
-// (24 bits; six products, 2^-25 left out) for f32 weights.  One term where the factors are already
+// 2^-16 of a product) for weights of 8 or 16 bits, whose own rounding is 2^-12 at best; three terms
+// (24 bits; six products, 2^-24 left out) for f32 weights.  One term where the factors are already
 // bf16, or both fp16.
 //
 // Operand layout.  v_mfma_f32_16x16x32 takes 8 consecutive k of row lane % 16 from each lane
@@ -49,12 +50,13 @@
 namespace {
 
 #define FSTX_GLOBAL __attribute__((address_space(1)))
+#define FSTX_LDS __attribute__((address_space(3)))
 typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
-constexpr uint32_t kTile = 128;  // rows and columns the packed factors are padded to: whole tiles of every type
+constexpr uint32_t kTile = 256;  // rows and columns the packed factors are padded to: whole tiles of every type and kernel
 constexpr uint32_t kBlk = 512;   // elements of one operand block (16 rows x 32 k)
 constexpr uint32_t kK = 32;      // k per block
 constexpr uint32_t kMaxJobs = 24;
@@ -119,6 +121,24 @@ __device__ __forceinline__ float bf16_term(float x) {
     return h;
 }
 
+__device__ __forceinline__ v8h half_terms(const float (&x)[8]) {
+    v8h h;
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) h[e] = (_Float16)x[e];
+    return h;
+}
+// the next bf16 term of eight values, which become what is left of them
+__device__ __forceinline__ v8b next_term(float (&x)[8]) {
+    v8b h;
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) {
+        const float f = bf16_term(x[e]);
+        h[e] = (__bf16)f;
+        x[e] = __builtin_isfinite(f) ? x[e] - f : 0.0f; // nothing behind an infinity or a NaN
+    }
+    return h;
+}
+
 // One wavefront per operand block, four per workgroup (a side has a multiple of eight blocks).
 __global__ __launch_bounds__(256) void pack_factors_kernel(const Jobs<PackJob> t) {
     const uint32_t ji = job_of(t, blockIdx.x);
@@ -135,23 +155,10 @@ __global__ __launch_bounds__(256) void pack_factors_kernel(const Jobs<PackJob> t
                    ? load_factor(job.src, (uint64_t)row * job.row_stride + (uint64_t)(k0 + e) * job.k_stride, job.type) : 0.0f;
     uint16_t *out = job.dst + ((uint64_t)lb * job.terms) * kBlk + lane * 8;
     if (job.half) {
-        v8h h;
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) h[e] = (_Float16)x[e];
-        *(FSTX_GLOBAL v8h *)out = h;
+        *(FSTX_GLOBAL v8h *)out = half_terms(x);
         return;
     }
-    for (uint32_t term = 0; term < job.terms; ++term) {
-        v8b h;
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-            const float f = bf16_term(x[e]);
-            h[e] = (__bf16)f;
-            // what is left for the next term; nothing behind an infinity or a NaN
-            x[e] = __builtin_isfinite(f) ? x[e] - f : 0.0f;
-        }
-        *(FSTX_GLOBAL v8b *)(out + term * kBlk) = h;
-    }
+    for (uint32_t term = 0; term < job.terms; ++term) *(FSTX_GLOBAL v8b *)(out + term * kBlk) = next_term(x);
 }
 
 template <uint32_t Cls> struct Operand { typedef v8b type; };
@@ -312,6 +319,18 @@ template <uint32_t T, uint32_t Cls, uint32_t NR = Tile<T>::kNR> struct Merge {
         }
     }
 
+    // what a lane's sums are multiplied with, per row
+    static __device__ __forceinline__ void scales(const MergeJob &job, uint32_t r0, uint32_t lane, float (&scale)[kNR]) {
+#pragma unroll
+        for (uint32_t i = 0; i < kNR; ++i) {
+            scale[i] = job.scale;
+            if constexpr (T == FSTX_F8_E4M3) {
+                const uint32_t row = r0 + 16 * i + (lane & 15), at = row < job.rows ? row : 0;
+                scale[i] = job.scale / *(const FSTX_GLOBAL float *)(job.weight_scale + (uint64_t)at * job.scale_step);
+            }
+        }
+    }
+
     static __device__ __forceinline__ void fetch(const uint16_t *at, uint64_t step, op_t (&f)[kTerms], uint32_t i) {
 #pragma unroll
         for (uint32_t p = 0; p < kTerms; ++p) f[p] = *(const FSTX_GLOBAL op_t *)(at + i * step + p * kBlk);
@@ -361,14 +380,7 @@ template <uint32_t T, uint32_t Cls, uint32_t NR = Tile<T>::kNR> struct Merge {
     template <uint32_t kHeld, bool Stream> static __device__ __forceinline__ void walk(const MergeJob &job, uint32_t r0, uint32_t first, uint32_t last, uint32_t lane) {
         constexpr uint32_t kH = kHeld ? kHeld : 1;
         float scale[kNR];
-#pragma unroll
-        for (uint32_t i = 0; i < kNR; ++i) {
-            scale[i] = job.scale;
-            if constexpr (T == FSTX_F8_E4M3) {
-                const uint32_t row = r0 + 16 * i + (lane & 15), at = row < job.rows ? row : 0;
-                scale[i] = job.scale / *(const FSTX_GLOBAL float *)(job.weight_scale + (uint64_t)at * job.scale_step);
-            }
-        }
+        scales(job, r0, lane, scale);
         const uint64_t step = (uint64_t)job.k_blocks * kTerms * kBlk;
         op_t held[kH][kNR][kTerms], d[kH][kNC][kTerms];
         if constexpr (kHeld > 0)
@@ -430,12 +442,147 @@ __global__ __launch_bounds__(64, 2) void low_rank_kernel(const uint32_t dies_log
     else Merge<T, Cls>::template walk<kHeld, false>(job, panel * Tile<T>::kRows, first, last, threadIdx.x);
 }
 
+// Longer products: four wavefronts (2 x 2 tiles) share the operands through LDS, 32 k at a time, the next ones on
+// their way while these are multiplied; a wavefront of its own would read both factors from L2 for each of its tiles. The
+// weights come last: another workgroup on the compute unit fills that time.
+template <uint32_t T, uint32_t Cls>
+__global__ __launch_bounds__(256, 2) void deep_low_rank_kernel(const uint32_t dies_log2, const Jobs<MergeJob> t) {
+    typedef Merge<T, Cls> M;
+    typedef typename M::op_t op_t;
+    constexpr uint32_t kTerms = M::kTerms, kNR = M::kNR, kNC = M::kNC;
+    constexpr uint32_t kUp = 2 * kNR * kTerms, kStage = kUp + 2 * kNC * kTerms; // operand blocks of a stage: rows', then columns'
+    __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * kStage * kBlk];
+    const uint32_t ji = job_of(t, blockIdx.x);
+    const MergeJob &job = t.job[ji];
+    uint32_t at;
+    if (!fstx_gather::tile_for_die(blockIdx.x - t.first[ji], job.n_walks, dies_log2, at)) return;
+    const uint32_t panel = at / job.walks, nth = at - panel * job.walks;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t step = (uint64_t)job.k_blocks * kTerms * kBlk;
+    const uint16_t *up = job.up + (uint64_t)panel * 2 * kNR * step + lane * 8, *down = job.down + (uint64_t)nth * 2 * kNC * step + lane * 8;
+    auto load_stage = [&](uint32_t kb, uint32_t buf) {
+#pragma unroll
+        for (uint32_t n = 0; n < kStage / 4; ++n) {
+            const uint32_t b = n * 4 + wave, in = b < kUp ? b : b - kUp;
+            const uint16_t *from = (b < kUp ? up : down) + in / kTerms * step + ((uint64_t)kb * kTerms + in % kTerms) * kBlk;
+            __builtin_amdgcn_global_load_lds((const FSTX_GLOBAL void *)from, (FSTX_LDS void *)(lds + (buf * kStage + b) * kBlk), 16, 0, 0);
+        }
+    };
+    v4f acc[kNR][kNC] = {};
+    load_stage(0, 0);
+    for (uint32_t kb = 0; kb < job.k_blocks; ++kb) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070); // this wavefront's loads have landed and its reads are done,
+        __builtin_amdgcn_s_barrier();       // and everybody's
+        asm volatile("" ::: "memory");
+        const uint16_t *base = lds + (kb & 1) * kStage * kBlk + lane * 8;
+        op_t u[kNR][kTerms], d[kNC][kTerms];
+#pragma unroll
+        for (uint32_t p = 0; p < kTerms; ++p) {
+#pragma unroll
+            for (uint32_t i = 0; i < kNR; ++i) u[i][p] = *(const op_t *)(base + (((wave >> 1) * kNR + i) * kTerms + p) * kBlk);
+#pragma unroll
+            for (uint32_t j = 0; j < kNC; ++j) d[j][p] = *(const op_t *)(base + (kUp + ((wave & 1) * kNC + j) * kTerms + p) * kBlk);
+        }
+        if (kb + 1 < job.k_blocks) load_stage(kb + 1, (kb + 1) & 1);
+        M::multiply(u, d, acc);
+    }
+    const uint32_t r0 = (panel * 2 + (wave >> 1)) * Tile<T>::kRows, c0 = (nth * 2 + (wave & 1)) * Tile<T>::kCols;
+    if (r0 >= job.rows || c0 >= job.cols) return; // (no barrier follows)
+    float scale[kNR];
+    M::scales(job, r0, lane, scale);
+    v4u w[kNR][2];
+    if (r0 + Tile<T>::kRows <= job.rows && c0 + Tile<T>::kCols <= job.cols) {
+        if (job.lines == 3) {
+            M::template load<false, true>(job, r0, c0, lane, w);
+            M::template finish<false, true>(job, r0, c0, lane, w, acc, scale);
+        } else {
+            M::template load<false, false>(job, r0, c0, lane, w);
+            M::template finish<false, false>(job, r0, c0, lane, w, acc, scale);
+        }
+    } else {
+        M::template load<true, false>(job, r0, c0, lane, w);
+        M::template finish<true, false>(job, r0, c0, lane, w, acc, scale);
+    }
+}
+
+// Few tiles and a rank of at most 32: a launch of its own for the factors would take as long as the merge.  Four wavefronts lay
+// out the operands of their common tile (64 rows of one line) in LDS and take 16 rows of it each.
+struct alignas(64) DirectJob {
+    MergeJob merge;
+    const char *up, *down;
+    uint64_t up_row, up_k, down_col, down_k; // strides, elements
+    uint32_t rank, up_type, down_type, pad;
+};
+static_assert(sizeof(DirectJob) == 192, "12 of them fit the kernel arguments");
+constexpr uint32_t kDirectJobs = 12;
+struct DirectJobs {
+    DirectJob job[kDirectJobs];
+    uint32_t first[kDirectJobs];
+};
+
+template <uint32_t T, uint32_t Cls> __global__ __launch_bounds__(256) void direct_low_rank_kernel(const DirectJobs t) {
+    typedef Merge<T, Cls, 1> M;
+    typedef typename M::op_t op_t;
+    constexpr uint32_t kTerms = M::kTerms, kNC = M::kNC, kBlocks = 4 + kNC;
+    __shared__ __attribute__((aligned(16))) uint16_t lds[kBlocks * kTerms * kBlk];
+    uint32_t ji = 0;
+#pragma unroll
+    for (uint32_t i = 1; i < kDirectJobs; ++i) ji += blockIdx.x >= t.first[i];
+    const DirectJob &job = t.job[ji];
+    const MergeJob &m = job.merge;
+    const uint32_t at = blockIdx.x - t.first[ji], panel = at / m.col_tiles, tile = at - panel * m.col_tiles;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rho = lane & 15, k0 = 8 * (lane >> 4);
+    const uint32_t r0 = panel * 64 + wave * 16, c0 = tile * Tile<T>::kCols;
+    const bool inside = r0 + 16 <= m.rows && c0 + Tile<T>::kCols <= m.cols;
+    v4u w[1][2];
+    if (inside) M::template load<false, false>(m, r0, c0, lane, w);
+    else M::template load<true, false>(m, r0, c0, lane, w);
+#pragma unroll
+    for (uint32_t n = 0; n < (kBlocks + 3) / 4; ++n) { // blocks of the rows' factor, then of the columns'
+        const uint32_t b = n * 4 + wave;
+        if (b >= kBlocks) break;
+        const bool cols = b >= 4;
+        const uint32_t row = cols ? c0 + column_of(b - 4, rho, M::kPer) : panel * 64 + b * 16 + rho;
+        const char *src = cols ? job.down : job.up;
+        const uint64_t row_stride = cols ? job.down_col : job.up_row, k_stride = cols ? job.down_k : job.up_k;
+        const uint32_t type = cols ? job.down_type : job.up_type;
+        const bool live = row < (cols ? m.cols : m.rows);
+        float x[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e)
+            x[e] = live && k0 + e < job.rank ? load_factor(src, (uint64_t)row * row_stride + (uint64_t)(k0 + e) * k_stride, type) : 0.0f;
+        uint16_t *out = lds + b * kTerms * kBlk + lane * 8;
+        if constexpr (Cls == kTermsH1) *(v8h *)out = half_terms(x);
+        else
+#pragma unroll
+            for (uint32_t p = 0; p < kTerms; ++p) *(v8b *)(out + p * kBlk) = next_term(x);
+    }
+    __syncthreads();
+    op_t u[1][kTerms], d[kNC][kTerms];
+#pragma unroll
+    for (uint32_t p = 0; p < kTerms; ++p) {
+        u[0][p] = *(const op_t *)(lds + (wave * kTerms + p) * kBlk + lane * 8);
+#pragma unroll
+        for (uint32_t j = 0; j < kNC; ++j) d[j][p] = *(const op_t *)(lds + ((4 + j) * kTerms + p) * kBlk + lane * 8);
+    }
+    v4f acc[1][kNC] = {};
+    M::multiply(u, d, acc);
+    float scale[1];
+    M::scales(m, r0, lane, scale);
+    if (inside) M::template finish<false, false>(m, r0, c0, lane, w, acc, scale);
+    else M::template finish<true, false>(m, r0, c0, lane, w, acc, scale);
+}
+
 // --------------------------------------------------------------- host side
 
 constexpr uint64_t kMaxSide = 0x7fffff00ull;    // rows, columns: positions stay in 32 bits
+// One launch without packing up to here: a [768, 2304] fp32 weight (864 tiles) 12 us instead of 16 with what the host does, three
+// fp16 ones of 2304 tiles 18.6 instead of 21.9; beyond it the tiles' own reads of the factors take more than that.
+constexpr uint64_t kDirectTiles = 4096;
 constexpr uint64_t kWaves = 4096;          // wavefronts that fill the device (eight per compute unit) twice
 constexpr uint64_t kLongestWalk = 4;
-constexpr uint64_t kLaunchBlocks = 48ull << 20; // workgroups of 64 lanes per launch: 32 bits of lanes
+constexpr uint64_t kLaunchBlocks = 12ull << 20; // workgroups of up to 256 lanes per launch: 32 bits of lanes
 
 inline uint32_t size_of(uint32_t type) { return type == FSTX_F32 ? 4 : type == FSTX_F8_E4M3 ? 1 : 2; }
 inline bool factor_type_ok(uint32_t t) { return t == FSTX_F32 || t == FSTX_F16 || t == FSTX_BF16; }
@@ -524,6 +671,7 @@ template <typename Job> void clear(Jobs<Job> &t) {
     for (uint32_t i = 0; i < kMaxJobs; ++i) t.first[i] = 0xffffffffu;
 }
 
+constexpr uint32_t kDeep = 3;
 // Blocks of 32 k of the rows' factor that stay in registers
 template <uint32_t T, uint32_t Cls> constexpr uint32_t held_most() { return Cls == kTermsB3 ? 1 : Cls == kTermsB2 ? 1 : 2; }
 
@@ -531,6 +679,7 @@ template <uint32_t T, uint32_t Cls> void launch(uint32_t grid, uint32_t held, co
     const uint32_t dies = fstx_internal::dies_log2();
     if (held == 1) hipLaunchKernelGGL((low_rank_kernel<T, Cls, 1>), dim3(grid), dim3(64), 0, s, dies, t);
     else if (held == 2 && held_most<T, Cls>() >= 2) hipLaunchKernelGGL((low_rank_kernel<T, Cls, held_most<T, Cls>() >= 2 ? 2 : 1>), dim3(grid), dim3(64), 0, s, dies, t);
+    else if (held == kDeep) hipLaunchKernelGGL((deep_low_rank_kernel<T, Cls>), dim3(grid), dim3(256), 0, s, dies, t);
     else hipLaunchKernelGGL((low_rank_kernel<T, Cls, 0>), dim3(grid), dim3(64), 0, s, dies, t);
 }
 
@@ -552,10 +701,25 @@ inline uint32_t on_lines(const fstx_low_rank_desc &d) {
     return ((((uint64_t)(uintptr_t)d.dst | dp) & 127) == 0 ? 1u : 0u) | ((((uint64_t)(uintptr_t)d.src | sp) & 127) == 0 ? 2u : 0u);
 }
 
-// which kernel variant serves a descriptor
+// Which kernel variant serves a descriptor: the number of blocks of the rows' factor that stay in registers, or 0 (walks
+// without), or kDeep.  [4096, 4096], walks against the deep kernel: bf16 weights, rank 96 24.0 / 22.7 us, 256 35.5 / 29.2, 512 52.6 /
+// 39.3; fp8, rank 256 34.2 / 22.7; f32 weights, which have half the products per byte and twice the bytes to bring,
+// rank 64 in three terms 41.0 / 48.4 and 128 53.5 / 56.1, rank 256 in one 47.8 / 50.0: from about 14 blocks times terms on.
 inline uint32_t held_of(const fstx_low_rank_desc &d) {
     const uint64_t kb = k_blocks_of(d), most = terms_of(class_of(d)) > 1 ? 1 : 2;
-    return kb == 0 ? 0 : kb <= most ? (uint32_t)kb : 0;
+    return kb <= most ? (uint32_t)kb : size_of(d.type) == 4 && kb * terms_of(class_of(d)) < 14 ? 0 : kDeep;
+}
+
+// Whether the whole call goes through direct_low_rank_kernel
+bool direct(const fstx_low_rank_desc *descs, uint32_t n) {
+    uint64_t tiles = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        const fstx_low_rank_desc &d = descs[i];
+        if (empty(d)) continue;
+        if (d.rank > kK) return false;
+        tiles += (d.rows + 63) / 64 * ((d.cols * size_of(d.type) + 127) / 128);
+    }
+    return tiles <= kDirectTiles;
 }
 
 } // namespace
@@ -563,17 +727,93 @@ inline uint32_t held_of(const fstx_low_rank_desc &d) {
 extern "C" int64_t fstx_merge_low_rank_workspace(const fstx_low_rank_desc *descs, uint32_t n) {
     const int rc = check(descs, n);
     if (rc < 0) return rc;
+    if (direct(descs, n)) return 0;
     uint64_t elems = 0;
     for (uint32_t i = 0; i < n; ++i)
         if (!empty(descs[i])) elems += packed_elems(descs[i].rows, descs[i]) + packed_elems(descs[i].cols, descs[i]);
     return (int64_t)(elems * 2);
 }
 
+namespace {
+
+template <uint32_t T, uint32_t Cls> void launch_direct(uint32_t grid, const DirectJobs &t, hipStream_t s) {
+    hipLaunchKernelGGL((direct_low_rank_kernel<T, Cls>), dim3(grid), dim3(256), 0, s, t);
+}
+
+int merge_direct(const fstx_low_rank_desc *descs, uint32_t n, hipStream_t s) {
+    uint64_t done = 0; // variants met so far
+    for (uint32_t first = 0; first < n; ++first) {
+        if (empty(descs[first])) continue;
+        const uint32_t type = descs[first].type, cls = class_of(descs[first]), variant = type * kTermClasses + cls;
+        if (done >> variant & 1) continue;
+        done |= 1ull << variant;
+        DirectJobs t;
+        for (uint32_t i = 0; i < kDirectJobs; ++i) t.first[i] = 0xffffffffu;
+        uint32_t k = 0;
+        uint64_t grid = 0;
+        auto flush = [&]() -> int {
+            if (k == 0) return 0;
+            fstx_internal::Range range("fstx direct_low_rank_kernel: %u jobs, %llu workgroups", k, (unsigned long long)grid);
+#define FSTX_CASE(T, C) case (T) * kTermClasses + (C): launch_direct<T, C>((uint32_t)grid, t, s); break;
+            switch (variant) {
+                FSTX_CASE(FSTX_F32, kTermsH1) FSTX_CASE(FSTX_F32, kTermsB1) FSTX_CASE(FSTX_F32, kTermsB3)
+                FSTX_CASE(FSTX_BF16, kTermsH1) FSTX_CASE(FSTX_BF16, kTermsB1) FSTX_CASE(FSTX_BF16, kTermsB2)
+                FSTX_CASE(FSTX_F16, kTermsH1) FSTX_CASE(FSTX_F16, kTermsB1) FSTX_CASE(FSTX_F16, kTermsB2)
+                FSTX_CASE(FSTX_F8_E4M3, kTermsH1) FSTX_CASE(FSTX_F8_E4M3, kTermsB1) FSTX_CASE(FSTX_F8_E4M3, kTermsB2)
+            default: break; // class_of gives no others
+            }
+#undef FSTX_CASE
+            k = 0;
+            grid = 0;
+            for (uint32_t i = 0; i < kDirectJobs; ++i) t.first[i] = 0xffffffffu;
+            return fstx_internal::check_launch("direct_low_rank_kernel");
+        };
+        for (uint32_t i = first; i < n; ++i) {
+            const fstx_low_rank_desc &d = descs[i];
+            if (empty(d) || d.type != type || class_of(d) != cls) continue;
+            if (k == kDirectJobs) {
+                const int rc = flush();
+                if (rc < 0) return rc;
+            }
+            const uint64_t size = size_of(type), col_tiles = (d.cols * size + 127) / 128;
+            DirectJob &j = t.job[k];
+            j = DirectJob{};
+            j.merge.dst = static_cast<char *>(d.dst);
+            j.merge.src = static_cast<const char *>(d.src);
+            j.merge.weight_scale = d.weight_scale;
+            j.merge.dst_pitch = d.dst_pitch * size;
+            j.merge.src_pitch = d.src_pitch * size;
+            j.merge.rows = (uint32_t)d.rows;
+            j.merge.cols = (uint32_t)d.cols;
+            j.merge.col_tiles = (uint32_t)col_tiles;
+            j.merge.scale = d.scale;
+            j.merge.scale_step = d.n_weight_scales > 1;
+            j.up = static_cast<const char *>(d.up);
+            j.down = static_cast<const char *>(d.down);
+            j.up_row = d.up_row_stride;
+            j.up_k = d.up_col_stride;
+            j.down_col = d.down_col_stride;
+            j.down_k = d.down_row_stride;
+            j.rank = (uint32_t)d.rank;
+            j.up_type = d.up_type;
+            j.down_type = d.down_type;
+            t.first[k++] = (uint32_t)grid;
+            grid += (d.rows + 63) / 64 * col_tiles;
+        }
+        const int rc = flush();
+        if (rc < 0) return rc;
+    }
+    return 0;
+}
+
+} // namespace
+
 extern "C" int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, void *workspace, uint64_t workspace_bytes, void *stream) {
     const int64_t need = fstx_merge_low_rank_workspace(descs, n);
     if (need < 0) return (int)need;
     if (need && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (uint64_t)need)) return -FSTX_E_INVAL;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (direct(descs, n)) return merge_direct(descs, n, s);
     uint16_t *const space = static_cast<uint16_t *>(workspace);
     { // factors -> operands
         Jobs<PackJob> t;
@@ -615,8 +855,8 @@ extern "C" int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, 
     // one launch (or a few) per kernel variant that occurs
     static const uint32_t types[4] = {FSTX_F32, FSTX_BF16, FSTX_F16, FSTX_F8_E4M3};
     const uint64_t dies = 1ull << fstx_internal::dies_log2();
-    for (uint32_t variant = 0; variant < 4 * kTermClasses * 3; ++variant) {
-        const uint32_t type = types[variant / (kTermClasses * 3)], cls = variant / 3 % kTermClasses, held = variant % 3;
+    for (uint32_t variant = 0; variant < 4 * kTermClasses * 4; ++variant) {
+        const uint32_t type = types[variant / (kTermClasses * 4)], cls = variant / 4 % kTermClasses, held = variant % 4;
         Jobs<MergeJob> t;
         clear(t);
         uint32_t k = 0;
@@ -630,7 +870,8 @@ extern "C" int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, 
             clear(t);
             return fstx_internal::check_launch("low_rank_kernel");
         };
-        const uint64_t size = size_of(type), tile_cols = 128 / size, tile_rows = size == 1 ? 32 : 64;
+        const uint64_t size = size_of(type), across = held == kDeep ? 2 : 1; // a deep workgroup's tile is two by two
+        const uint64_t tile_cols = across * 128 / size, tile_rows = across * (size == 1 ? 32 : 64);
         uint64_t tiles = 0; // of the whole call, for the length of the walks
         for (uint32_t i = 0; i < n; ++i)
             if (!empty(descs[i])) tiles += (descs[i].cols + tile_cols - 1) / tile_cols * ((descs[i].rows + tile_rows - 1) / tile_rows);
@@ -642,7 +883,7 @@ extern "C" int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, 
             if (d.type != type || class_of(d) != cls || held_of(d) != held) continue;
             const uint64_t col_tiles = (d.cols + tile_cols - 1) / tile_cols, panels = (d.rows + tile_rows - 1) / tile_rows;
             uint64_t walk = tiles / kWaves;
-            walk = walk < 1 ? 1 : walk > kLongestWalk ? kLongestWalk : walk;
+            walk = held == kDeep || walk < 1 ? 1 : walk > kLongestWalk ? kLongestWalk : walk;
             const uint64_t walks = (col_tiles + walk - 1) / walk;
             const uint64_t blocks = (panels * walks + dies - 1) / dies * dies;
             if (k == kMaxJobs || grid + blocks > kLaunchBlocks) {

@@ -15,7 +15,7 @@ tensor.
 
 import re
 from collections import OrderedDict
-from typing import Any, Dict, List, Optional, Tuple
+from typing import Any, Dict, List, Optional, Sequence, Tuple
 
 from .common import init_logger
 from .frameworks import FrameworkOpBase, ProcessGroupBase, TensorBase
@@ -257,4 +257,41 @@ class FilesBufferOnDevice:
         self.framework.merge_adapters(items, alpha, scale, fan_in_fan_out)
         for name, factory in zip(names, factories):
             factory.shuffled.pop(name, None)  # a shard kept from before the merge is not this weight's any more
+        return names
+
+    def merge_checkpoints(
+        self, others: Sequence["FilesBufferOnDevice"], scale: float = 1.0, orthogonal: Optional[Sequence[str]] = None
+    ) -> List[str]:
+        """Merge the fine-tuned checkpoints ``others`` into the base checkpoint held here, in place.
+        Returns the names of the tensors that changed: those the others hold (all of them the same ones).
+
+        With ``D`` the sum of the others' differences to the base, a tensor named in ``orthogonal``
+        (default: every one of two dimensions, both larger than 1) becomes ``W + scale * s * O``, ``O`` being
+        the orthogonal matrix nearest to ``D`` and ``s`` the mean of ``D``'s singular values: every direction that some
+        checkpoint changed weighs the same, so that the strong directions of one task do not drown
+        the others.  The remaining tensors get the mean difference, ``W + scale * D / len(others)``.
+
+        fp32, fp16 and bf16 tensors of the same type and shape everywhere; everything is checked before the
+        first one changes, all work is queued on the current stream."""
+        if not others:
+            raise ValueError("merge_checkpoints: no checkpoints to merge")
+        names = list(others[0].key_to_rank_lidx)
+        for other in others:
+            if set(other.key_to_rank_lidx) != set(names):
+                raise ValueError("merge_checkpoints: the checkpoints do not hold the same tensors")
+        missing = [n for n in (*names, *(orthogonal or ())) if n not in self.key_to_rank_lidx or n not in others[0].key_to_rank_lidx]
+        if missing:
+            raise ValueError(f"merge_checkpoints: {missing[0]} was not found in files")
+        items, factories = [], []
+        for name in names:
+            factory = self._factory(name)[2]
+            base = factory._held(name, "merge_checkpoints")
+            tuned = [o._factory(name)[2]._held(name, "merge_checkpoints") for o in others]
+            shape = self.get_shape(name)
+            square = name in orthogonal if orthogonal is not None else len(shape) == 2 and min(shape) > 1
+            items.append((base, tuned, square))
+            factories.append(factory)
+        self.framework.merge_checkpoints(items, scale)
+        for name, factory in zip(names, factories):
+            factory.shuffled.pop(name, None)
         return names

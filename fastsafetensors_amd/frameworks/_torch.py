@@ -27,7 +27,7 @@ import torch
 from .. import _native
 from ..common import SingleGroup, TensorFrame
 from ..st_types import Device, DeviceType, DType, dtype_size
-from ..updates import LowRankUpdate, merge_low_rank
+from ..updates import POLAR_COEFFICIENTS, LowRankUpdate, merge_low_rank, orthogonalize
 from . import FrameworkOpBase, ProcessGroupBase, TensorBase
 
 dtype_convert: Dict[DType, torch.dtype] = {
@@ -56,6 +56,9 @@ need_workaround_dtypes: Dict[DType, DType] = {
     DType.F8_E8M0: DType.U8,
     DType.F4: DType.U8,
 }
+
+# elements of the matrices whose updates are orthogonalised in one call: 1 GiB of fp32 updates
+_MERGE_ELEMS = 256 * 1024 * 1024
 
 
 @dataclass
@@ -526,6 +529,40 @@ class TorchOp(FrameworkOpBase):
             updates.append(LowRankUpdate(weight.real_tensor, up, down, s,
                                          None if weight_scale is None else weight_scale.real_tensor))
         merge_low_rank(updates)
+
+    def merge_checkpoints(self, items: List[Tuple[TorchTensor, List[TorchTensor], bool]], scale: float) -> None:
+        work = []
+        for base, tuned, orthogonal in items:
+            w, ts = base.real_tensor, [t.real_tensor for t in tuned]
+            if w.dtype not in (torch.float32, torch.float16, torch.bfloat16) or any(t.dtype != w.dtype for t in ts):
+                raise TypeError(f"merge_checkpoints serves fp32, fp16 and bf16 tensors of one type, not {[str(x.dtype) for x in (w, *ts)]}")
+            if any(t.shape != w.shape for t in ts):
+                raise ValueError(f"shapes do not match: {[tuple(x.shape) for x in (w, *ts)]}")
+            if orthogonal and w.dim() != 2:
+                raise ValueError(f"a tensor of shape {tuple(w.shape)} cannot be orthogonalised")
+            work.append((w, ts, orthogonal))
+
+        def delta(w: torch.Tensor, ts: List[torch.Tensor]) -> torch.Tensor:
+            out = torch.zeros(w.shape, dtype=torch.float32, device=w.device)
+            for t in ts:
+                out += t.float() - w.float()
+            return out
+
+        with torch.no_grad():
+            for w, ts, orthogonal in work:
+                if not orthogonal and w.numel():
+                    w.copy_(w.float() + delta(w, ts) * (scale / len(ts)))
+            matrices = [(w, ts) for w, ts, orthogonal in work if orthogonal and w.numel()]
+            while matrices:  # as many at a time as fit next to the checkpoints
+                group, elems = [], 0
+                while matrices and (not group or elems + matrices[0][0].numel() <= _MERGE_ELEMS):
+                    group.append(matrices.pop(0))
+                    elems += group[-1][0].numel()
+                deltas = [delta(w, ts) for w, ts in group]
+                for (w, _), d, o in zip(group, deltas, orthogonalize(deltas, coefficients=POLAR_COEFFICIENTS)):
+                    # sum of the singular values = <d, o>; their mean keeps the update's size
+                    mean = (d * o).sum() / min(w.shape)
+                    w.copy_(w.float() + o * (scale * mean))
 
     # ---- misc ------------------------------------------------------------------
     def synchronize(self, device: Device) -> None:

@@ -3,8 +3,8 @@
 
 The reference only moves weights (its users merge adapters with the framework's own products);
 here the merge runs as a streaming pass over the loaded weights.  ``merge_low_rank`` is what
-``FilesBufferOnDevice.merge_adapter`` calls; it takes any tensors on the GPU.  ``orthogonalize``
-replaces an update by its nearest orthogonal matrix.
+``FilesBufferOnDevice.merge_adapter`` calls, ``orthogonalize`` -- the nearest orthogonal matrix of an
+update -- what ``FilesBufferOnDevice.merge_checkpoints`` does; both take any tensors on the GPU.
 """
 
 import contextlib
@@ -218,6 +218,9 @@ def merge_low_rank(updates: Sequence[LowRankUpdate]) -> List[torch.Tensor]:
 # largest into about 0.7 .. 1.2: the slope at zero is as steep as a quintic's can be without leaving that range
 DEFAULT_COEFFICIENTS = ((3.4445, -4.7750, 2.0315),) * 5
 
+# ... followed by steps with a fixed point of third order at 1: singular values from about 1/400 of the largest up end at 1
+POLAR_COEFFICIENTS = DEFAULT_COEFFICIENTS + ((1.875, -1.25, 0.375),) * 4
+
 
 def orthogonalize(
     updates: Union[torch.Tensor, Sequence[torch.Tensor]],
@@ -237,7 +240,7 @@ def orthogonalize(
     product is a small part of the sum, and in the last step of a bf16 update.
 
     The default coefficients leave singular values between 0.7 and 1.2, which is what an optimiser needs;
-    appending a few ``(1.875, -1.25, 0.375)`` steps drives them to 1.  Coefficients must keep the
+    ``POLAR_COEFFICIENTS`` drives them to 1.  Coefficients must keep the
     iterates' singular values below about 2.  There is no gradient: tensors that require one are refused while
     gradients are being recorded."""
     single = isinstance(updates, torch.Tensor)

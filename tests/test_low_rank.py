@@ -40,12 +40,15 @@ def test_header_and_binding_list_the_same_functions_and_layouts(tmp_path):
 def test_workspace_sizes():
     assert need() == 0
     assert need(desc(rows=0)) == need(desc(cols=0)) == need(desc(rank=0, up=None, down=None)) == 0
-    # 100 x 60 at rank 8: (128 + 128) rows of 32 k, 2 bytes, one term
-    assert need(desc()) == 256 * 32 * 2
-    assert need(desc(ftype=F32)) == 2 * 256 * 32 * 2
-    assert need(desc(ftype=F32, type=F32)) == 3 * 256 * 32 * 2
-    assert need(desc(rank=33)) == 256 * 64 * 2
-    assert need(desc(), desc(dst=0x2000000)) == 2 * 256 * 32 * 2
+    assert need(desc()) == 0  # few tiles, a small rank: no packed factors
+    # 100 x 60 at rank 64, padded to (256 + 256) rows of 64 k, 2 bytes, one term
+    assert need(desc(rank=64)) == 512 * 64 * 2
+    assert need(desc(rank=64, ftype=F32)) == 2 * 512 * 64 * 2
+    assert need(desc(rank=64, ftype=F32, type=F32)) == 3 * 512 * 64 * 2
+    assert need(desc(rank=33)) == 512 * 64 * 2
+    assert need(desc(rank=64), desc(dst=0x2000000)) == 512 * (64 + 32) * 2
+    far = 1 << 44
+    assert need(desc(rows=1 << 15, cols=1 << 15, up=far, down=2 * far)) == (2 << 15) * 32 * 2
 
 
 @pytest.mark.parametrize("bad", [
@@ -72,8 +75,8 @@ def test_sizes_out_of_range_are_refused():
 
 
 def test_workspace_must_be_there_aligned_and_large_enough():
-    arr = (_native.FstxLowRankDesc * 1)(desc())
-    fn, size = _native.lib().fstx_merge_low_rank, need(desc())
+    arr = (_native.FstxLowRankDesc * 1)(desc(rank=64))
+    fn, size = _native.lib().fstx_merge_low_rank, need(desc(rank=64))
     assert fn(arr, 1, None, size, None) == INVAL
     assert fn(arr, 1, 0x5000010, size, None) == INVAL
     assert fn(arr, 1, 0x5000000, size - 1, None) == INVAL
@@ -87,15 +90,15 @@ def test_overlaps_between_updates():
     assert need(a, desc(dst=0x1000000 + 60 * 2 * 50)) == INVAL          # rows in common
     assert need(a, desc(dst=0x3000000, src=0x1000000)) == INVAL         # one reads what the other writes
     assert need(a, desc(dst=0x3000000, up=0x1000000 + 64)) == INVAL
-    assert need(a, desc(dst=0x1000000 + 100 * 60 * 2)) > 0              # side by side
+    assert need(a, desc(dst=0x1000000 + 100 * 60 * 2)) >= 0              # side by side
     # column blocks of one tensor with rows of 120
     left, right = desc(pitch=120), desc(dst=0x1000000 + 120, pitch=120)
-    assert need(left, right) > 0 and need(right, left) > 0
+    assert need(left, right) >= 0 and need(right, left) >= 0
     assert need(left, desc(dst=0x1000000 + 118, pitch=120)) == INVAL    # one column in common
     assert need(desc(dst=0x1000000 + 118, pitch=120), left) == INVAL
-    assert need(right, desc(dst=0x1000000 + 240, pitch=120)) > 0        # the next row's left block
+    assert need(right, desc(dst=0x1000000 + 240, pitch=120)) >= 0        # the next row's left block
     assert need(right, desc(dst=0x1000000 + 242, pitch=120)) == INVAL   # ... running into the row after it
-    assert need(desc(dst=0x1000000, src=0x1000000 + 120, pitch=120)) > 0  # out of place between two column blocks
+    assert need(desc(dst=0x1000000, src=0x1000000 + 120, pitch=120)) >= 0  # out of place between two column blocks
 
 
 def test_python_refuses_what_is_not_in_gpu_memory():

@@ -33,9 +33,10 @@ def make(m, n, r, wt, ut, dt, seed=0):
 
 
 def check(got, w, u, d, s, wt, ut, dt, ws=None):
-    """``got`` (on the GPU) against w + s u d of the host tensors, in 64 bits."""
-    w64, u64, d64 = w.double(), u.double(), d.double()
-    held = torch.ones(()) if ws is None else ws.double().reshape(-1, 1) if ws.numel() > 1 else ws.double().reshape(())
+    """``got`` (on the GPU) against w + s u d of the host tensors, in 64 bits (there, too)."""
+    w64, u64, d64 = (t.to(got.device).double() for t in (w, u, d))
+    ws = None if ws is None else ws.to(got.device)
+    held = torch.ones((), device=got.device) if ws is None else ws.double().reshape(-1, 1) if ws.numel() > 1 else ws.double().reshape(())
     want = w64 + s * (u64 @ d64) / held
     bound = abs(s) * (u64.abs() @ d64.abs()) / held
     r = u.shape[1]
@@ -45,7 +46,7 @@ def check(got, w, u, d, s, wt, ut, dt, ws=None):
     if wt == "e4m3":
         want = want.clamp(-448.0, 448.0)
     tol = (want.abs() + slack) * (torch.finfo(T[wt]).eps / 2) + HALF_SUBNORMAL[wt] + slack
-    got = got.cpu().double()
+    got = got.double()
     assert got.shape == want.shape
     bad = ~((got - want).abs() <= tol)
     assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), (got - want)[bad][:4], tol[bad][:4])
@@ -79,10 +80,36 @@ def test_large_ranks_and_many_tiles(dev, wt):
         check(got, w, u, d, 0.5, wt, "bf16", "bf16", ws)
 
 
+@pytest.mark.parametrize("ut,dt", [("bf16", "bf16"), ("f32", "f32")])
 @pytest.mark.parametrize("wt", ["f32", "f16", "bf16", "e4m3"])
-def test_pitched_and_misaligned_weights_leave_their_surroundings_alone(dev, wt):
+def test_ranks_that_go_through_shared_operands(dev, wt, ut, dt):
+    """Ranks from the first that the walking kernel leaves to another on, with edges on both sides."""
+    for m, n, r in ((1, 300, 97), (129, 1, 160), (130, 517, 161), (257, 255, 449), (300, 333, 1000)):
+        w, u, d = make(m, n, r, wt, ut, dt)
+        ws = torch.rand(m) + 0.5 if wt == "e4m3" else None
+        (got,) = merge_low_rank([LowRankUpdate(w.to(dev), u.to(dev), d.to(dev), 0.5, None if ws is None else ws.to(dev))])
+        check(got, w, u, d, 0.5, wt, ut, dt, ws)
+
+
+@pytest.mark.parametrize("r", [5, 33])
+@pytest.mark.parametrize("wt", ["f32", "f16", "bf16", "e4m3"])
+def test_long_walks_with_edges(dev, wt, r):
+    """More tiles than the one-launch kernel takes: walks of several tiles, the last panel and the last tile of each cut off."""
+    n = {"f32": 2047, "f16": 4095, "bf16": 4095, "e4m3": 8189}[wt]
+    w, u, d = make(5003, n, r, wt, "bf16", "bf16")
+    ws = torch.rand(5003) + 0.5 if wt == "e4m3" else None
+    (got,) = merge_low_rank([LowRankUpdate(w.to(dev), u.to(dev), d.to(dev), 0.5, None if ws is None else ws.to(dev))])
+    check(got, w, u, d, 0.5, wt, "bf16", "bf16", ws)
+    w, u, d = make(5056, n + 64 - n % 64, r, wt, "bf16", "bf16")  # ... and whole lines throughout
+    (got,) = merge_low_rank([LowRankUpdate(w.to(dev), u.to(dev), d.to(dev), 0.5, None if ws is None else torch.ones(1, device=dev))])
+    check(got, w, u, d, 0.5, wt, "bf16", "bf16", None if ws is None else torch.ones(1))
+
+
+@pytest.mark.parametrize("wt", ["f32", "f16", "bf16", "e4m3"])
+@pytest.mark.parametrize("r", [7, 40, 200])
+def test_pitched_and_misaligned_weights_leave_their_surroundings_alone(dev, wt, r):
     """A column block of a wider tensor at every element offset of a 16-byte vector, in place and out of place."""
-    m, n, r, size = 70, 131, 7, T[wt].itemsize
+    m, n, size = 70, 131, T[wt].itemsize
     w, u, d = make(m, n, r, wt, "bf16", "bf16")
     ws = torch.tensor(1.25) if wt == "e4m3" else None
     wsd = None if ws is None else ws.to(dev)
