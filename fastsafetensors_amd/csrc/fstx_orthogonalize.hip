@@ -649,6 +649,202 @@ __global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Dea
     finish_block<kPhase, Terms>(job, c, rb, cb, v, there, threadIdx.x);
 }
 
+// ------------------------------------------------------------ slim matrices
+//
+// Up to 32 rows the whole iteration fits one workgroup when it is done on the Gram matrix M = G G^T in 64 bits: X is Q G with
+// Q a polynomial of M, so that a step is P = a I + b A + c A^2, Q <- P Q, A <- P A P, which all commute.  Squaring the
+// singular values costs half of the digits, which 64 bits have to spare and two fp16 terms have not: of a [1, 1] fp32
+// update they got 1.6e-6 of the value wrong, and this 4e-8.  It is three launches whatever the number of steps, and reads the
+// update twice: with five steps a [1, 700] fp32 update takes 22 us instead of 101, [32, 4096] 31 instead of 119 and
+// [32, 28672] 50 instead of 287.  At 64 rows one workgroup's products would take as long as the launches they save.
+// The partial sums of M are added in a fixed order.
+
+constexpr uint32_t kSlim = 32;      // rows at most
+constexpr uint32_t kSlimJobs = 32;
+constexpr uint32_t kSlimParts = 128; // workgroups that share the columns of one matrix
+
+struct alignas(32) SlimJob {
+    const char *src;
+    char *dst;
+    double *grams; // n_parts of kSlim x kSlim
+    double *q;     // kSlim x kSlim
+    uint64_t x_row, x_col, dst_pitch; // elements, elements, bytes
+    uint32_t p, q_cols, type, flipped, n_parts, pad;
+};
+struct SlimJobs {
+    SlimJob job[kSlimJobs];
+    uint32_t first[kSlimJobs];
+};
+static_assert(sizeof(SlimJobs) <= 3328, "fits the kernel arguments");
+
+__device__ __forceinline__ uint32_t slim_job_of(const SlimJobs &t, uint32_t b) {
+    uint32_t ji = 0;
+#pragma unroll
+    for (uint32_t i = 1; i < kSlimJobs; ++i) ji += b >= t.first[i];
+    return ji;
+}
+
+// v_mfma_f64_16x16x4: lane l holds A[l % 16][l / 16] and B[l / 16][l % 16], and D[4 r + l / 16][l % 16] in element r.
+using f64x4 = __attribute__((__vector_size__(4 * sizeof(double)))) double;
+__device__ __forceinline__ f64x4 mfma64(double a, double b, f64x4 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+
+// A workgroup's share of M, 64 columns at a time, the next ones on their way while these are multiplied; a wave takes 16 of
+// them and the tiles on and below the diagonal.
+__global__ __launch_bounds__(256) void slim_gram_kernel(const SlimJobs t) {
+    constexpr uint32_t kWide = 64, kLoads = kSlim * kWide / 256;
+    __shared__ union {
+        float x[kSlim][kWide + 4];
+        double sums[4][256];
+    } lds;
+    const uint32_t ji = slim_job_of(t, blockIdx.x);
+    const SlimJob &job = t.job[ji];
+    const uint32_t me = blockIdx.x - t.first[ji], p = job.p, n = job.q_cols, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const bool across = job.x_row < job.x_col; // columns of X lie along memory
+    float next[kLoads];
+    auto at = [&](uint32_t k, uint32_t &i, uint32_t &c) {
+        const uint32_t e = threadIdx.x + 256 * k;
+        i = across ? e % kSlim : e / kWide;
+        c = across ? e / kSlim : e % kWide;
+    };
+    auto load = [&](uint64_t c0) {
+#pragma unroll
+        for (uint32_t k = 0; k < kLoads; ++k) {
+            uint32_t i, c;
+            at(k, i, c);
+            next[k] = i < p && c0 + c < n ? load_elem(job.src, i * job.x_row + (c0 + c) * job.x_col, job.type) : 0.0f;
+        }
+    };
+    f64x4 acc[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+    const uint64_t stride = (uint64_t)job.n_parts * kWide;
+    load((uint64_t)me * kWide);
+    for (uint64_t c0 = (uint64_t)me * kWide; c0 < n; c0 += stride) {
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < kLoads; ++k) {
+            uint32_t i, c;
+            at(k, i, c);
+            lds.x[i][c] = next[k];
+        }
+        __syncthreads();
+        if (c0 + stride < n) load(c0 + stride);
+#pragma unroll
+        for (uint32_t k = 0; k < 16; k += 4) {
+            const double a = lds.x[lane % 16][wave * 16 + k + lane / 16];
+            acc[0] = mfma64(a, a, acc[0]);
+            if (p > 16) {
+                const double b = lds.x[16 + lane % 16][wave * 16 + k + lane / 16];
+                acc[1] = mfma64(b, a, acc[1]);
+                acc[2] = mfma64(b, b, acc[2]);
+            }
+        }
+    }
+    double *out = job.grams + (uint64_t)me * kSlim * kSlim;
+#pragma unroll
+    for (uint32_t tile = 0; tile < 3; ++tile) { // the waves' sums, in order
+        __syncthreads();
+        for (uint32_t r = 0; r < 4; ++r) lds.sums[wave][(4 * r + lane / 16) * 16 + lane % 16] = acc[tile][r];
+        __syncthreads();
+        const uint32_t i = threadIdx.x / 16 + (tile > 0 ? 16 : 0), j = threadIdx.x % 16 + (tile > 1 ? 16 : 0);
+        const double sum = lds.sums[0][threadIdx.x] + lds.sums[1][threadIdx.x] + lds.sums[2][threadIdx.x] + lds.sums[3][threadIdx.x];
+        out[i * kSlim + j] = sum;
+        if (tile == 1) out[j * kSlim + i] = sum;
+    }
+}
+
+struct Steps {
+    float c[3 * 64];
+    uint32_t n;
+    float eps;
+};
+
+// One workgroup per matrix: Q.  Rows and columns from p on are zero throughout (those of P are not, but meet only zeros).
+__global__ __launch_bounds__(512) void slim_steps_kernel(const SlimJobs t, const Steps steps) {
+    using Matrix = double[kSlim][kSlim + 1];
+    __shared__ Matrix a, q, m, w;
+    const SlimJob &job = t.job[blockIdx.x];
+    const uint32_t p = job.p, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const uint32_t i0 = wave / 2 % 2 * 16, j0 = wave % 2 * 16, row = i0 + lane / 16, col = j0 + lane % 16;
+    for (uint32_t e = threadIdx.x; e < kSlim * kSlim; e += 512) {
+        double sum = 0;
+#pragma unroll 8
+        for (uint32_t k = 0; k < job.n_parts; ++k) sum += job.grams[(uint64_t)k * kSlim * kSlim + e];
+        a[e / kSlim][e % kSlim] = sum;
+    }
+    __syncthreads();
+    double trace = 0;
+    for (uint32_t i = 0; i < p; ++i) trace += a[i][i];
+    const double factor = 1.0 / (sqrt(trace) + (double)steps.eps);
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < kSlim * kSlim; e += 512) {
+        a[e / kSlim][e % kSlim] *= factor * factor;
+        q[e / kSlim][e % kSlim] = e / kSlim == e % kSlim && e % kSlim < p ? factor : 0.0;
+    }
+    __syncthreads();
+    // a wave's tile of x y; all of these are symmetric, so that y's rows serve as its columns
+    auto product = [&](const Matrix &x, const Matrix &y) {
+        f64x4 d = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t k = 0; k < kSlim; k += 4) d = mfma64(x[i0 + lane % 16][k + lane / 16], y[j0 + lane % 16][k + lane / 16], d);
+        return d;
+    };
+    const bool first = wave < 4;
+    const bool mine = i0 < p && j0 < p;
+    for (uint32_t s = 0; s < steps.n; ++s) {
+        const double ca = steps.c[3 * s], cb = steps.c[3 * s + 1], cc = steps.c[3 * s + 2];
+        f64x4 d;
+        if (first) {
+            d = product(a, a);
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r)
+                m[row + 4 * r][col] = (row + 4 * r == col ? ca : 0.0) + cb * a[row + 4 * r][col] + cc * d[r];
+        }
+        __syncthreads();
+        if (mine) d = first ? product(m, q) : product(m, a);
+        __syncthreads();
+        if (mine) {
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) (first ? q : w)[row + 4 * r][col] = d[r];
+        }
+        __syncthreads();
+        if (first && mine) {
+            d = product(w, m);
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) a[row + 4 * r][col] = d[r];
+        }
+        __syncthreads();
+    }
+    for (uint32_t e = threadIdx.x; e < kSlim * kSlim; e += 512) job.q[e] = q[e / kSlim][e % kSlim];
+}
+
+// The result, Q G: 16 columns by wave, read whole before they are written
+__global__ __launch_bounds__(256) void slim_apply_kernel(const SlimJobs t) {
+    const uint32_t ji = slim_job_of(t, blockIdx.x);
+    const SlimJob &job = t.job[ji];
+    const uint32_t p = job.p, lane = threadIdx.x % 64, from = lane / 16;
+    const uint64_t c = (uint64_t)(blockIdx.x - t.first[ji]) * 64 + threadIdx.x / 64 * 16 + lane % 16;
+    double g[kSlim / 4];
+#pragma unroll
+    for (uint32_t k = 0; k < kSlim / 4; ++k)
+        g[k] = 4 * k + from < p && c < job.q_cols ? load_elem(job.src, (4 * k + from) * job.x_row + c * job.x_col, job.type) : 0.0f;
+#pragma unroll
+    for (uint32_t i0 = 0; i0 < kSlim; i0 += 16) {
+        if (i0 >= p) break;
+        f64x4 d = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t k = 0; k < kSlim / 4; ++k) d = mfma64(job.q[(i0 + lane % 16) * kSlim + 4 * k + from], g[k], d);
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r) {
+            const uint64_t i = i0 + 4 * r + from;
+            if (i >= p || c >= job.q_cols) continue;
+            char *at = job.dst + (job.flipped ? c : i) * job.dst_pitch;
+            const uint64_t along = job.flipped ? i : c;
+            if (job.type == FSTX_F32) ((FSTX_GLOBAL float *)at)[along] = (float)d[r];
+            else if (job.type == FSTX_BF16) ((FSTX_GLOBAL __bf16 *)at)[along] = (__bf16)(float)d[r];
+            else ((FSTX_GLOBAL half_t *)at)[along] = (half_t)(float)d[r];
+        }
+    }
+}
+
 // --------------------------------------------------------------- host side
 
 constexpr uint64_t kMaxSide = 1u << 20;
@@ -658,6 +854,7 @@ constexpr uint32_t kMaxSteps = 64;
 inline bool type_ok(uint32_t t) { return t == FSTX_F32 || t == FSTX_F16 || t == FSTX_BF16; }
 inline uint32_t size_of(uint32_t t) { return t == FSTX_F32 ? 4 : 2; }
 inline bool empty(const fstx_orthogonalize_desc &d) { return d.rows == 0 || d.cols == 0; }
+inline bool slim(const fstx_orthogonalize_desc &d) { return !empty(d) && (d.rows < d.cols ? d.rows : d.cols) <= kSlim; }
 
 struct Sides {
     uint64_t p, q, pp, qp;
@@ -686,6 +883,9 @@ int check(const fstx_orthogonalize_desc *descs, uint32_t n) {
         if ((d.src_row_stride | d.src_col_stride | d.dst_pitch) >> 40) return -FSTX_E_RANGE;
         if (!d.dst || !d.src || (uintptr_t)d.dst % size_of(d.type) || (uintptr_t)d.src % size_of(d.type)) return -FSTX_E_INVAL;
         if (d.rows > 1 && d.dst_pitch < d.cols) return -FSTX_E_INVAL;
+        // exactly in place, or apart
+        const bool in_place = d.dst == d.src && (d.rows == 1 || d.src_row_stride == d.dst_pitch) && (d.cols == 1 || d.src_col_stride == 1);
+        if (!in_place && dst_of(d).meets(src_of(d))) return -FSTX_E_INVAL;
     }
     for (uint32_t i = 0; i < n; ++i)
         for (uint32_t j = 0; j < n; ++j)
@@ -892,7 +1092,7 @@ uint32_t next_set(const fstx_orthogonalize_desc *descs, uint32_t n, const float 
     set->n = 0;
     for (uint32_t k = 0; k < kMaxJobs; ++k) set->t.first[k] = 0xffffffffu;
     for (uint32_t i = first; i < n; ++i) {
-        if (empty(descs[i]) || one_term_steps(descs[i], coefficients, steps) != kind) continue;
+        if (empty(descs[i]) || slim(descs[i]) || one_term_steps(descs[i], coefficients, steps) != kind) continue;
         const uint64_t need = Sides(descs[i]).bytes();
         if (set->n == kMaxJobs || (set->n && *bytes + need > kChunkBytes)) return i;
         set->add(descs[i], at + *bytes);
@@ -905,8 +1105,61 @@ uint32_t next_set(const fstx_orthogonalize_desc *descs, uint32_t n, const float 
 bool taken(const fstx_orthogonalize_desc *descs, uint32_t i, const float *coefficients, uint32_t steps) {
     const uint64_t kind = one_term_steps(descs[i], coefficients, steps);
     for (uint32_t j = 0; j < i; ++j)
-        if (!empty(descs[j]) && one_term_steps(descs[j], coefficients, steps) == kind) return true;
+        if (!empty(descs[j]) && !slim(descs[j]) && one_term_steps(descs[j], coefficients, steps) == kind) return true;
     return false;
+}
+
+// Slim matrices from `first` on, as many as one set of launches takes; returns where the next set begins.
+uint32_t slim_set(const fstx_orthogonalize_desc *descs, uint32_t n, uint32_t first, char *at, SlimJobs *t, uint64_t *bytes) {
+    uint32_t k = 0;
+    *bytes = 0;
+    if (t)
+        for (uint32_t i = 0; i < kSlimJobs; ++i) {
+            t->first[i] = 0xffffffffu;
+            t->job[i] = SlimJob{};
+        }
+    for (uint32_t i = first; i < n; ++i) {
+        const fstx_orthogonalize_desc &d = descs[i];
+        if (!slim(d)) continue;
+        if (k == kSlimJobs) return i;
+        const bool flipped = d.rows > d.cols;
+        const uint64_t p = flipped ? d.cols : d.rows, q = flipped ? d.rows : d.cols, parts = (q + 255) / 256;
+        const uint32_t n_parts = (uint32_t)(parts < kSlimParts ? parts : kSlimParts);
+        if (t) {
+            double *space = reinterpret_cast<double *>(at + *bytes);
+            t->job[k] = SlimJob{static_cast<const char *>(d.src), static_cast<char *>(d.dst), space + kSlim * kSlim, space,
+                                flipped ? d.src_col_stride : d.src_row_stride, flipped ? d.src_row_stride : d.src_col_stride,
+                                d.dst_pitch * size_of(d.type), (uint32_t)p, (uint32_t)q, d.type, flipped, n_parts, 0};
+        }
+        *bytes += (uint64_t)(n_parts + 1) * kSlim * kSlim * sizeof(double);
+        ++k;
+    }
+    return n;
+}
+
+int slim_launch(SlimJobs &t, const float *coefficients, uint32_t count, float eps, hipStream_t stream) {
+    Steps steps = {};
+    for (uint32_t i = 0; i < 3 * count; ++i) steps.c[i] = coefficients[i];
+    steps.n = count;
+    steps.eps = eps;
+    uint32_t n = 0, grid = 0;
+    for (; n < kSlimJobs && t.job[n].p; ++n) {
+        t.first[n] = grid;
+        grid += t.job[n].n_parts;
+    }
+    fstx_internal::Range range("fstx slim kernels: %u matrices", n);
+    hipLaunchKernelGGL(slim_gram_kernel, dim3(grid), dim3(256), 0, stream, t);
+    int rc = fstx_internal::check_launch("slim_gram_kernel");
+    if (rc < 0) return rc;
+    hipLaunchKernelGGL(slim_steps_kernel, dim3(n), dim3(512), 0, stream, t, steps);
+    if ((rc = fstx_internal::check_launch("slim_steps_kernel")) < 0) return rc;
+    grid = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        t.first[i] = grid;
+        grid += (t.job[i].q_cols + 63) / 64;
+    }
+    hipLaunchKernelGGL(slim_apply_kernel, dim3(grid), dim3(256), 0, stream, t);
+    return fstx_internal::check_launch("slim_apply_kernel");
 }
 
 } // namespace
@@ -916,8 +1169,13 @@ extern "C" int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *d
     if (rc < 0) return rc;
     if (steps < 1 || steps > kMaxSteps || !coefficients) return -FSTX_E_INVAL;
     uint64_t most = 0;
+    for (uint32_t first = 0; first < n;) {
+        uint64_t bytes;
+        first = slim_set(descs, n, first, nullptr, nullptr, &bytes);
+        if (bytes > most) most = bytes;
+    }
     for (uint32_t i = 0; i < n; ++i) {
-        if (empty(descs[i]) || taken(descs, i, coefficients, steps)) continue;
+        if (empty(descs[i]) || slim(descs[i]) || taken(descs, i, coefficients, steps)) continue;
         for (uint32_t first = i; first < n;) {
             Launcher set;
             set.d.dies_log2 = fstx_internal::dies_log2();
@@ -938,8 +1196,16 @@ extern "C" int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t
     if (need < 0) return (int)need;
     if (!(eps >= 0)) return -FSTX_E_INVAL;
     if (need && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (uint64_t)need)) return -FSTX_E_INVAL;
+    for (uint32_t first = 0; first < n;) {
+        SlimJobs t;
+        uint64_t bytes;
+        first = slim_set(descs, n, first, static_cast<char *>(workspace), &t, &bytes);
+        if (bytes == 0) continue;
+        const int rc = slim_launch(t, coefficients, steps, eps, static_cast<hipStream_t>(stream));
+        if (rc < 0) return rc;
+    }
     for (uint32_t i = 0; i < n; ++i) {
-        if (empty(descs[i]) || taken(descs, i, coefficients, steps)) continue;
+        if (empty(descs[i]) || slim(descs[i]) || taken(descs, i, coefficients, steps)) continue;
         for (uint32_t first = i; first < n;) {
             Launcher set;
             set.d.dies_log2 = fstx_internal::dies_log2();

@@ -29,12 +29,15 @@ def size(p, q):
 
 def test_workspace_sizes():
     assert need() == 0 and need(desc(rows=0)) == 0 and need(desc(cols=0)) == 0
-    # operands padded to 256 x 128, and at most one round of workgroups' partial sums (512 tiles of 256 x 128)
-    for rows, cols, p, q in ((100, 300, 256, 384), (300, 100, 256, 384), (1, 1, 256, 128), (1000, 2500, 1024, 2560)):
+    # operands padded to 256 x 256, and at most one round of workgroups' partial sums (512 tiles of 256 x 128)
+    for rows, cols, p, q in ((100, 300, 256, 512), (300, 100, 256, 512), (33, 33, 256, 256), (1000, 2500, 1024, 2560)):
         got = need(desc(rows=rows, cols=cols))
         assert size(p, q) <= got <= size(p, q) + 512 * 256 * 128 * 4
+    # up to 32 rows: the Gram matrix in parts of 256 columns, at most 128 of them
+    assert need(desc(rows=1, cols=1)) == 2 * 8192 and need(desc(rows=32, cols=1000)) == 5 * 8192
+    assert need(desc(rows=1 << 20, cols=5, strides=(5, 1), src=1 << 40)) == 129 * 8192
     small = [desc(dst=BASE + (i << 20), src=2 * BASE + (i << 20)) for i in range(50)]
-    assert 20 * size(256, 384) <= need(*small) < 21 * size(256, 384) + 512 * 256 * 128 * 4  # twenty at a time
+    assert 20 * size(256, 512) <= need(*small) < 21 * size(256, 512) + 512 * 256 * 128 * 4  # twenty at a time
     large = [desc(dst=(i + 1) << 36, src=(i + 100) << 36, rows=16384, cols=16384) for i in range(3)]
     assert size(16384, 16384) <= need(*large) < 2 * size(16384, 16384)   # one at a time
 
@@ -54,6 +57,9 @@ def test_overlaps():
     assert need(a, desc(src=3 * BASE)) == INVAL                  # one destination twice
     assert need(a, desc(dst=2 * BASE)) == INVAL                  # a destination that another update reads
     assert need(desc(dst=BASE, src=BASE), desc(dst=3 * BASE)) > 0  # an update may be its own destination
+    assert need(desc(dst=BASE, src=BASE + 2)) == INVAL           # but only exactly
+    assert need(desc(dst=BASE, src=BASE, pitch=400)) == INVAL
+    assert need(desc(dst=BASE, src=BASE, strides=(1, 100))) == INVAL
 
 
 def test_steps_eps_and_workspace_are_checked():

@@ -70,6 +70,17 @@ def test_shapes_and_types(dev, dt):
         check(got, g, dt)
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_slim_matrices(dev, dt):
+    """Up to 32 rows or columns everything is done in 64 bits: what is left is the rounding of the result."""
+    shapes = [(1, 1), (1, 2), (2, 1), (3, 255), (8, 256), (257, 9), (16, 16), (17, 4099), (5000, 31), (32, 32), (32, 70001), (100003, 2)]
+    mats = [make(m, n, i).to(T[dt]) for i, (m, n) in enumerate(shapes)]
+    for g, got in zip(mats, orthogonalize([g.to(dev) for g in mats], coefficients=POLAR)):
+        want = iterate(g, POLAR)
+        # half a step of the type of every element, and a 64-bit calculation's own 2^-40 or so of the largest
+        assert ((got.cpu().double() - want).abs() <= want.abs() * (torch.finfo(T[dt]).eps / 2 * 1.001) + 2.0**-25 + want.abs().max() * 2.0**-40).all(), g.shape
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("m,n", [(1024, 4096), (2048, 2048), (5000, 1100), (1500, 1500)])
 def test_large_tiles(dev, dt, m, n):
