@@ -40,11 +40,13 @@
 // Two lanes of neighbouring rows trade their halves of the two lines (trade), and W moves
 // between memory and the accumulator layout 16 bytes per lane and a whole line per row and instruction.
 
+#include <errno.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "fstx_gather_core.h"
 #include "fstx_internal.h"
+#include "fstx_overlap.h"
 #include "fstx_update.h"
 
 namespace {
@@ -597,31 +599,11 @@ inline uint32_t class_of(const fstx_low_rank_desc &d) {
 
 inline bool empty(const fstx_low_rank_desc &d) { return d.rows == 0 || d.cols == 0; }
 
-// a block of bytes: `rows` segments of `width` bytes, `pitch` apart
-struct Block {
-    uint64_t at, width, pitch, rows;
-    uint64_t end() const { return at + (rows - 1) * pitch + width; }
-};
-
-bool overlap(const Block &a, const Block &b) {
-    if (a.at >= b.end() || b.at >= a.end()) return false;
-    if (a.pitch != b.pitch || a.rows == 1 || b.rows == 1) return true; // spans that touch: not told apart further
-    if (b.at < a.at) return overlap(b, a);
-    // rows of one tensor: b starts `shift` rows and `col` bytes behind a
-    const uint64_t shift = (b.at - a.at) / a.pitch, col = (b.at - a.at) % a.pitch;
-    if (shift < a.rows && col < a.width) return true;
-    return shift + 1 < a.rows && col + b.width > a.pitch; // b's rows run on into a's next rows
-}
-
-Block block_of(const void *p, uint64_t rows, uint64_t cols, uint64_t pitch, uint64_t size) {
-    return Block{(uint64_t)(uintptr_t)p, cols * size, (rows == 1 ? cols : pitch) * size, rows};
-}
+using fstx_overlap::Block;
+using fstx_overlap::block_of;
 Block dst_of(const fstx_low_rank_desc &d) { return block_of(d.dst, d.rows, d.cols, d.dst_pitch, size_of(d.type)); }
 Block src_of(const fstx_low_rank_desc &d) { return block_of(d.src, d.rows, d.cols, d.src_pitch, size_of(d.type)); }
-Block factor_of(const void *p, uint64_t n0, uint64_t s0, uint64_t n1, uint64_t s1, uint32_t type) {
-    const uint64_t last = (n0 - 1) * s0 + (n1 - 1) * s1 + 1;
-    return Block{(uint64_t)(uintptr_t)p, last * size_of(type), last * size_of(type), 1};
-}
+constexpr uint64_t kMaxSpan = 1ull << 48; // elements from a matrix's first to its last
 
 int check(const fstx_low_rank_desc *descs, uint32_t n) {
     if (n && !descs) return -FSTX_E_INVAL;
@@ -638,6 +620,7 @@ int check(const fstx_low_rank_desc *descs, uint32_t n) {
             if (!d.up || !d.down || (uintptr_t)d.up % size_of(d.up_type) || (uintptr_t)d.down % size_of(d.down_type)) return -FSTX_E_INVAL;
             if ((d.up_row_stride | d.up_col_stride | d.down_row_stride | d.down_col_stride) >> 31) return -FSTX_E_RANGE;
         }
+        if (d.rows > 1 && ((d.dst_pitch > d.src_pitch ? d.dst_pitch : d.src_pitch) > kMaxSpan / d.rows)) return -FSTX_E_RANGE;
         const bool eight = d.type == FSTX_F8_E4M3;
         if (eight ? !d.weight_scale || (uintptr_t)d.weight_scale % 4 || (d.n_weight_scales != 1 && d.n_weight_scales != d.rows)
                   : d.weight_scale != nullptr || d.n_weight_scales != 0)
@@ -646,20 +629,22 @@ int check(const fstx_low_rank_desc *descs, uint32_t n) {
         if (tiles > kLaunchBlocks / 2 || (blocks16(d.rows) + blocks16(d.cols)) * k_blocks_of(d) > kLaunchBlocks / 2) return -FSTX_E_RANGE;
         // in place, or a source that the destination does not touch
         const bool in_place = d.dst == d.src && (d.rows == 1 || d.dst_pitch == d.src_pitch);
-        if (!in_place && overlap(dst_of(d), src_of(d))) return -FSTX_E_INVAL;
+        if (!in_place && fstx_overlap::overlap(dst_of(d), src_of(d))) return -FSTX_E_INVAL;
     }
+    fstx_overlap::List list(5ull * n);
+    if (!list.at) return -ENOMEM;
     for (uint32_t i = 0; i < n; ++i) {
-        if (empty(descs[i])) continue;
-        const Block out = dst_of(descs[i]);
-        for (uint32_t j = 0; j < n; ++j) {
-            const fstx_low_rank_desc &d = descs[j];
-            if (empty(d)) continue;
-            if (j != i && ((j > i && overlap(out, dst_of(d))) || overlap(out, src_of(d)))) return -FSTX_E_INVAL;
-            if (d.rank && (overlap(out, factor_of(d.up, d.rows, d.up_row_stride, d.rank, d.up_col_stride, d.up_type)) ||
-                           overlap(out, factor_of(d.down, d.rank, d.down_row_stride, d.cols, d.down_col_stride, d.down_type))))
-                return -FSTX_E_INVAL;
+        const fstx_low_rank_desc &d = descs[i];
+        if (empty(d)) continue;
+        list.add(dst_of(d), i, fstx_overlap::kWritten);
+        list.add(src_of(d), i, fstx_overlap::kSource);
+        if (d.rank) {
+            list.add(block_of(d.up, d.rows, d.up_row_stride, d.rank, d.up_col_stride, size_of(d.up_type)), i, fstx_overlap::kRead);
+            list.add(block_of(d.down, d.rank, d.down_row_stride, d.cols, d.down_col_stride, size_of(d.down_type)), i, fstx_overlap::kRead);
         }
+        if (d.weight_scale) list.add(block_of(d.weight_scale, 1, d.n_weight_scales, 0, sizeof(float)), i, fstx_overlap::kRead);
     }
+    if (fstx_overlap::any_conflict(list.at, list.n)) return -FSTX_E_INVAL;
     return 0;
 }
 

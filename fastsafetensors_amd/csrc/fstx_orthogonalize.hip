@@ -33,12 +33,14 @@
 // at the diagonal) is made in registers by an MFMA with the identity, which is exact.
 // Sides are padded with zeros to whole tiles; products of zeros stay zeros, nothing is masked.
 
+#include <errno.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
 #include "fstx_gather_core.h"
 #include "fstx_internal.h"
+#include "fstx_overlap.h"
 #include "fstx_update.h"
 
 namespace {
@@ -863,15 +865,10 @@ struct Sides {
     uint64_t bytes() const { return (3 * pp * qp + 2 * pp * pp) * 2 * sizeof(half_t) + kPartials * sizeof(double); }
 };
 
-// span of bytes a strided matrix lies in
-struct Span {
-    uint64_t at, end;
-    Span(const void *p, uint64_t rows, uint64_t rs, uint64_t cols, uint64_t cs, uint64_t size)
-        : at((uint64_t)(uintptr_t)p), end(at + ((rows - 1) * rs + (cols - 1) * cs + 1) * size) {}
-    bool meets(const Span &o) const { return at < o.end && o.at < end; }
-};
-Span dst_of(const fstx_orthogonalize_desc &d) { return Span(d.dst, d.rows, d.dst_pitch, d.cols, 1, size_of(d.type)); }
-Span src_of(const fstx_orthogonalize_desc &d) { return Span(d.src, d.rows, d.src_row_stride, d.cols, d.src_col_stride, size_of(d.type)); }
+using fstx_overlap::Block;
+using fstx_overlap::block_of;
+Block dst_of(const fstx_orthogonalize_desc &d) { return block_of(d.dst, d.rows, d.cols, d.dst_pitch, size_of(d.type)); }
+Block src_of(const fstx_orthogonalize_desc &d) { return block_of(d.src, d.rows, d.src_row_stride, d.cols, d.src_col_stride, size_of(d.type)); }
 
 int check(const fstx_orthogonalize_desc *descs, uint32_t n) {
     if (n && !descs) return -FSTX_E_INVAL;
@@ -885,13 +882,16 @@ int check(const fstx_orthogonalize_desc *descs, uint32_t n) {
         if (d.rows > 1 && d.dst_pitch < d.cols) return -FSTX_E_INVAL;
         // exactly in place, or apart
         const bool in_place = d.dst == d.src && (d.rows == 1 || d.src_row_stride == d.dst_pitch) && (d.cols == 1 || d.src_col_stride == 1);
-        if (!in_place && dst_of(d).meets(src_of(d))) return -FSTX_E_INVAL;
+        if (!in_place && fstx_overlap::overlap(dst_of(d), src_of(d))) return -FSTX_E_INVAL;
     }
-    for (uint32_t i = 0; i < n; ++i)
-        for (uint32_t j = 0; j < n; ++j)
-            if (i != j && !empty(descs[i]) && !empty(descs[j]) &&
-                (dst_of(descs[i]).meets(dst_of(descs[j])) || dst_of(descs[i]).meets(src_of(descs[j]))))
-                return -FSTX_E_INVAL;
+    fstx_overlap::List list(2ull * n);
+    if (!list.at) return -ENOMEM;
+    for (uint32_t i = 0; i < n; ++i) {
+        if (empty(descs[i])) continue;
+        list.add(dst_of(descs[i]), i, fstx_overlap::kWritten);
+        list.add(src_of(descs[i]), i, fstx_overlap::kSource);
+    }
+    if (fstx_overlap::any_conflict(list.at, list.n)) return -FSTX_E_INVAL;
     return 0;
 }
 
@@ -1101,13 +1101,27 @@ uint32_t next_set(const fstx_orthogonalize_desc *descs, uint32_t n, const float 
     return n;
 }
 
-// whether an earlier descriptor is of the same kind (and its sets have taken this one)
-bool taken(const fstx_orthogonalize_desc *descs, uint32_t i, const float *coefficients, uint32_t steps) {
-    const uint64_t kind = one_term_steps(descs[i], coefficients, steps);
-    for (uint32_t j = 0; j < i; ++j)
-        if (!empty(descs[j]) && !slim(descs[j]) && one_term_steps(descs[j], coefficients, steps) == kind) return true;
-    return false;
-}
+// The first descriptor from `from` on that begins the sets of another kind (`n`: there is none).  Kinds met so far are
+// kept; behind the last one that there is room for, the earlier descriptors are looked through.
+struct Kinds {
+    uint64_t met[32];
+    uint32_t n = 0;
+    uint32_t next(const fstx_orthogonalize_desc *descs, uint32_t count, const float *coefficients, uint32_t steps, uint32_t from) {
+        for (uint32_t i = from; i < count; ++i) {
+            if (empty(descs[i]) || slim(descs[i])) continue;
+            const uint64_t kind = one_term_steps(descs[i], coefficients, steps);
+            bool taken = false;
+            for (uint32_t k = 0; k < n; ++k) taken = taken || met[k] == kind;
+            if (!taken && n < 32) {
+                met[n++] = kind;
+                return i;
+            }
+            for (uint32_t j = 0; j < i && !taken; ++j) taken = !empty(descs[j]) && !slim(descs[j]) && one_term_steps(descs[j], coefficients, steps) == kind;
+            if (!taken) return i;
+        }
+        return count;
+    }
+};
 
 // Slim matrices from `first` on, as many as one set of launches takes; returns where the next set begins.
 uint32_t slim_set(const fstx_orthogonalize_desc *descs, uint32_t n, uint32_t first, char *at, SlimJobs *t, uint64_t *bytes) {
@@ -1168,14 +1182,16 @@ extern "C" int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *d
     const int rc = check(descs, n);
     if (rc < 0) return rc;
     if (steps < 1 || steps > kMaxSteps || !coefficients) return -FSTX_E_INVAL;
+    for (uint32_t k = 0; k < 3 * steps; ++k)
+        if (!isfinite(coefficients[k])) return -FSTX_E_INVAL;
     uint64_t most = 0;
     for (uint32_t first = 0; first < n;) {
         uint64_t bytes;
         first = slim_set(descs, n, first, nullptr, nullptr, &bytes);
         if (bytes > most) most = bytes;
     }
-    for (uint32_t i = 0; i < n; ++i) {
-        if (empty(descs[i]) || slim(descs[i]) || taken(descs, i, coefficients, steps)) continue;
+    Kinds kinds;
+    for (uint32_t i = 0; (i = kinds.next(descs, n, coefficients, steps, i)) < n; ++i) {
         for (uint32_t first = i; first < n;) {
             Launcher set;
             set.d.dies_log2 = fstx_internal::dies_log2();
@@ -1194,7 +1210,7 @@ extern "C" int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t
                                   void *workspace, uint64_t workspace_bytes, void *stream) {
     const int64_t need = fstx_orthogonalize_workspace(descs, n, coefficients, steps);
     if (need < 0) return (int)need;
-    if (!(eps >= 0)) return -FSTX_E_INVAL;
+    if (!(eps >= 0) || !isfinite(eps)) return -FSTX_E_INVAL;
     if (need && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (uint64_t)need)) return -FSTX_E_INVAL;
     for (uint32_t first = 0; first < n;) {
         SlimJobs t;
@@ -1204,8 +1220,8 @@ extern "C" int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t
         const int rc = slim_launch(t, coefficients, steps, eps, static_cast<hipStream_t>(stream));
         if (rc < 0) return rc;
     }
-    for (uint32_t i = 0; i < n; ++i) {
-        if (empty(descs[i]) || slim(descs[i]) || taken(descs, i, coefficients, steps)) continue;
+    Kinds kinds;
+    for (uint32_t i = 0; (i = kinds.next(descs, n, coefficients, steps, i)) < n; ++i) {
         for (uint32_t first = i; first < n;) {
             Launcher set;
             set.d.dies_log2 = fstx_internal::dies_log2();

@@ -27,7 +27,7 @@ import torch
 from .. import _native
 from ..common import SingleGroup, TensorFrame
 from ..st_types import Device, DeviceType, DType, dtype_size
-from ..updates import POLAR_COEFFICIENTS, LowRankUpdate, merge_low_rank, orthogonalize
+from ..updates import MAX_SHORT_SIDE, MAX_SIDE, POLAR_COEFFICIENTS, LowRankUpdate, merge_low_rank, orthogonalize
 from . import FrameworkOpBase, ProcessGroupBase, TensorBase
 
 dtype_convert: Dict[DType, torch.dtype] = {
@@ -531,6 +531,8 @@ class TorchOp(FrameworkOpBase):
         merge_low_rank(updates)
 
     def merge_checkpoints(self, items: List[Tuple[TorchTensor, List[TorchTensor], bool]], scale: float) -> None:
+        if not math.isfinite(scale):
+            raise ValueError(f"merge_checkpoints: scale is {scale}")
         work = []
         for base, tuned, orthogonal in items:
             w, ts = base.real_tensor, [t.real_tensor for t in tuned]
@@ -538,8 +540,10 @@ class TorchOp(FrameworkOpBase):
                 raise TypeError(f"merge_checkpoints serves fp32, fp16 and bf16 tensors of one type, not {[str(x.dtype) for x in (w, *ts)]}")
             if any(t.shape != w.shape for t in ts):
                 raise ValueError(f"shapes do not match: {[tuple(x.shape) for x in (w, *ts)]}")
-            if orthogonal and w.dim() != 2:
-                raise ValueError(f"a tensor of shape {tuple(w.shape)} cannot be orthogonalised")
+            if any(t.device != w.device for t in ts):
+                raise ValueError(f"the checkpoints are on different devices: {[str(x.device) for x in (w, *ts)]}")
+            if orthogonal and (w.dim() != 2 or not w.is_cuda or max(w.shape) > MAX_SIDE or min(w.shape) > MAX_SHORT_SIDE):
+                raise ValueError(f"a tensor of shape {tuple(w.shape)} on {w.device} cannot be orthogonalised")
             work.append((w, ts, orthogonal))
 
         def delta(w: torch.Tensor, ts: List[torch.Tensor]) -> torch.Tensor:

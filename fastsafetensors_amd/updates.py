@@ -96,6 +96,9 @@ def _low_rank_desc(u: LowRankUpdate, device: torch.device, grad: bool) -> _nativ
         raise ValueError(f"shapes do not match: weight {tuple(w.shape)}, up {tuple(up.shape)}, down {tuple(down.shape)}")
     if out.shape != w.shape or out.dtype != w.dtype:
         raise ValueError(f"out is {tuple(out.shape)} {out.dtype}, weight {tuple(w.shape)} {w.dtype}")
+    scale = float(u.scale)
+    if not abs(scale) <= _LARGEST:
+        raise ValueError(f"scale is {u.scale}, not a finite 32-bit number")
     n_scales, ws_at = 0, None
     if w.dtype == torch.float8_e4m3fn:
         if ws is None:
@@ -121,19 +124,20 @@ def _low_rank_desc(u: LowRankUpdate, device: torch.device, grad: bool) -> _nativ
         out.data_ptr(), w.data_ptr(), up.data_ptr(), down.data_ptr(), ws_at,
         w.shape[0], w.shape[1], r, _pitch(out, "out"), _pitch(w, "weight"),
         up.stride(0), up.stride(1), down.stride(0), down.stride(1),
-        float(u.scale), _WEIGHT_TYPES[w.dtype], _FACTOR_TYPES[up.dtype], _FACTOR_TYPES[down.dtype], n_scales, 0,
+        scale, _WEIGHT_TYPES[w.dtype], _FACTOR_TYPES[up.dtype], _FACTOR_TYPES[down.dtype], n_scales, 0,
     )
 
 
 _DESC = struct.Struct("=14Qf5I")  # fstx_low_rank_desc
 assert _DESC.size == _native.ctypes.sizeof(_native.FstxLowRankDesc)
+_LARGEST = torch.finfo(torch.float32).max
 _E4M3 = _WEIGHT_TYPES[torch.float8_e4m3fn]
 
 
 def _pack_plain(buf: bytearray, at: int, u: LowRankUpdate, device: torch.device, grad: bool) -> bool:
     """Write the descriptor of an update with nothing unusual about it; False where ``_low_rank_desc`` has to look (and
     to say what is wrong).  A call costs a few microseconds per update on the host, as much as a small merge on the GPU."""
-    w, up, down, ws, out = u.weight, u.up, u.down, u.weight_scale, u.out
+    w, up, down, ws, out, scale = u.weight, u.up, u.down, u.weight_scale, u.out, u.scale
     try:
         if out is None:
             out = w
@@ -143,7 +147,7 @@ def _pack_plain(buf: bytearray, at: int, u: LowRankUpdate, device: torch.device,
         (m, n), (m2, r), (r2, n2) = w.shape, up.shape, down.shape
         (src_pitch, one), (dst_pitch, out_one) = w.stride(), out.stride()
         if (
-            m != m2 or n != n2 or r != r2 or one != 1 or out_one != 1 or src_pitch < n or dst_pitch < n
+            not -_LARGEST <= scale <= _LARGEST or m != m2 or n != n2 or r != r2 or one != 1 or out_one != 1 or src_pitch < n or dst_pitch < n
             or w.device != device or up.device != device or down.device != device
             or (grad and (w.requires_grad or up.requires_grad or down.requires_grad))
         ):
@@ -157,7 +161,7 @@ def _pack_plain(buf: bytearray, at: int, u: LowRankUpdate, device: torch.device,
         else:
             ws_at, n_scales = 0, 0
         _DESC.pack_into(buf, at, out.data_ptr(), w.data_ptr(), up.data_ptr(), down.data_ptr(), ws_at, m, n, r, dst_pitch, src_pitch,
-                        *up.stride(), *down.stride(), u.scale, wt, ut, dt, n_scales, 0)
+                        *up.stride(), *down.stride(), scale, wt, ut, dt, n_scales, 0)
         return True
     except (AttributeError, KeyError, TypeError, ValueError, RuntimeError, struct.error):
         return False
@@ -222,22 +226,29 @@ DEFAULT_COEFFICIENTS = ((3.4445, -4.7750, 2.0315),) * 5
 POLAR_COEFFICIENTS = DEFAULT_COEFFICIENTS + ((1.875, -1.25, 0.375),) * 4
 
 
+# sides that fstx_orthogonalize takes: the longer and the shorter one
+MAX_SIDE, MAX_SHORT_SIDE = 1 << 20, 1 << 16
+
+
 def orthogonalize(
     updates: Union[torch.Tensor, Sequence[torch.Tensor]],
     coefficients: Sequence[Sequence[float]] = DEFAULT_COEFFICIENTS,
     eps: float = 1e-7,
     outs: Optional[Sequence[torch.Tensor]] = None,
 ) -> Union[torch.Tensor, List[torch.Tensor]]:
-    """The nearest orthogonal matrix of every update (fp32, fp16 or bf16, two dimensions, any strides),
-    approximated by Newton-Schulz steps on ``X = G / (|G|_F + eps)``: for each ``(a, b, c)``
+    """The nearest orthogonal matrix of every update (fp32, fp16 or bf16, two dimensions, any strides,
+    up to 2^20 a side, the shorter one up to 2^16) approximated by Newton-Schulz steps on ``X = G / (|G|_F + eps)``: for each ``(a, b, c)``
     ``X <- a X + (b A + c A^2) X`` with ``A = X X^T`` (the shorter side as rows).
 
     Returns new tensors of the updates' shapes and types, or fills ``outs`` (contiguous rows or
-    contiguous columns; an update may be its own ``out``).  One tensor in, one tensor out; a sequence gives a list.
+    contiguous columns; an update may be its own ``out``, but not overlap it partly).  One tensor in, one tensor out; a sequence gives a list.
     The matrices of one call run together, so that small ones share launches.  All are checked before
     anything runs.  The iterates are held in 22 bits and products are as accurate as 32-bit ones, except where
     shorter operands (11 bits) cannot be told from that in a result of the update's type: in steps in which the
     product is a small part of the sum, and in the last step of a bf16 update.
+
+    Up to 32 rows or columns everything is done in 64 bits.  A call takes 12 bytes of workspace per element of its matrices and
+    8 per element of their squares, up to 4 GiB and more only for a matrix that alone needs more.
 
     The default coefficients leave singular values between 0.7 and 1.2, which is what an optimiser needs;
     ``POLAR_COEFFICIENTS`` drives them to 1.  Coefficients must keep the
@@ -250,6 +261,8 @@ def orthogonalize(
         raise ValueError("coefficients must be 1 to 64 triples (a, b, c)")
     if not all(math.isfinite(v) for v in flat) or not (math.isfinite(eps) and eps >= 0):
         raise ValueError("coefficients must be finite, eps finite and not negative")
+    if not all(abs(v) <= _LARGEST for v in (*flat, eps)):
+        raise ValueError("coefficients and eps must be 32-bit numbers")
     if outs is not None:
         outs = [outs] if single and isinstance(outs, torch.Tensor) else list(outs)
         if len(outs) != len(mats):

@@ -24,11 +24,13 @@ extern "C" {
 /* dst = round(src + scale * (up @ down)); dst == src (same pitch) merges in place.
  * Products and sums are held in 32 bits; factors of f32 are split into bf16 terms, as many as the
  * weight's type can tell apart.  With FSTX_F8_E4M3 weights W stands for W * weight_scale[row] and the
- * result is (W * weight_scale + scale * up @ down) / weight_scale, saturated to +-448 (a NaN stays one). */
+ * result is (W * weight_scale + scale * up @ down) / weight_scale, saturated to +-448 (a NaN stays one).
+ * An infinity in a factor makes its row or column infinite or NaN.  Up to 2^31 - 256 rows and columns and about
+ * 6 * 10^9 elements (-FSTX_E_RANGE). */
 typedef struct fstx_low_rank_desc {
     void *dst;                  /* [rows, cols] elements of `type`, rows dst_pitch elements apart       */
     const void *src;            /* [rows, cols] elements of `type`, rows src_pitch elements apart       */
-    const void *up;             /* [rows, rank] of `up_type`, any strides (elements, not negative)      */
+    const void *up;             /* [rows, rank] of `up_type`, any strides (elements, below 2^31)         */
     const void *down;           /* [rank, cols] of `down_type`                                          */
     const float *weight_scale;  /* device memory, FSTX_F8_E4M3 only: 1 or `rows` floats                 */
     uint64_t rows, cols, rank;
@@ -47,7 +49,7 @@ typedef struct fstx_low_rank_desc {
 int64_t fstx_merge_low_rank_workspace(const fstx_low_rank_desc *descs, uint32_t n);
 
 /* Any number of merges in a few launches.  No destination may overlap another destination, another
- * descriptor's source or any factor (column blocks of one tensor do not overlap). */
+ * descriptor's source, any factor or weight scale (column blocks of one tensor do not overlap). */
 int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, void *workspace,
                         uint64_t workspace_bytes, void *stream);
 
@@ -56,10 +58,11 @@ int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, void *works
  * with the shorter side as rows (orthogonal rows if rows <= cols, else orthogonal columns).  Iterates are
  * held in 22 bits and products as accurate as 32-bit ones, shorter operands only where a result of the
  * type cannot tell; sums are held in 32 bits, the norm's in 64.  While the steps run the
- * iterates' singular values have to stay below about 2 (those of X start at 1 or less). */
+ * iterates' singular values have to stay below about 2 (those of X start at 1 or less).  With up to 32 rows
+ * or columns everything is done in 64 bits.  An infinity or a NaN anywhere makes the whole result NaN. */
 typedef struct fstx_orthogonalize_desc {
     void *dst;                              /* [rows, cols] of `type`, rows dst_pitch elements apart     */
-    const void *src;                        /* [rows, cols] of `type`, any strides (elements); may be dst */
+    const void *src;                        /* [rows, cols] of `type`, any strides (elements); dst or apart */
     uint64_t rows, cols;                    /* up to 2^20, the smaller one up to 2^16                    */
     uint64_t dst_pitch;
     uint64_t src_row_stride, src_col_stride;
@@ -72,8 +75,8 @@ int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *descs, uint3
                                      uint32_t steps);
 
 /* Any number of matrices; those that fit one set of launches together run together.  `coefficients`
- * (host memory) are a, b, c of each of the 1..64 steps.  No destination may overlap another
- * descriptor's source or destination. */
+ * (host memory) are a, b, c of each of the 1..64 steps, all finite.  No destination may overlap another
+ * descriptor's source or destination, or its own source partly. */
 int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t n, const float *coefficients, uint32_t steps,
                        float eps, void *workspace, uint64_t workspace_bytes, void *stream);
 

@@ -101,6 +101,42 @@ def test_overlaps_between_updates():
     assert need(desc(dst=0x1000000, src=0x1000000 + 120, pitch=120)) >= 0  # out of place between two column blocks
 
 
+def test_weight_scales_are_not_written_over():
+    assert need(desc(type=E4M3, ws=0x7000000, n_ws=100)) >= 0
+    assert need(desc(type=E4M3, ws=0x1000000 + 400, n_ws=1)) == INVAL
+    assert need(desc(), desc(dst=0x3000000, type=E4M3, ws=0x1000000 + 100 * 60 * 2 - 4, n_ws=100)) == INVAL
+
+
+def test_spans_beyond_memory_are_refused():
+    assert need(desc(rows=1 << 20, cols=8, pitch=1 << 39)) == RANGE
+
+
+def test_overlaps_among_thousands_of_updates():
+    """Blocks of columns of one tensor, whole tensors and factors, in any order; one overlap anywhere is found."""
+    import random
+
+    descs = [desc(dst=(1 << 40) + i * 12000, up=(1 << 41) + i * 1600, down=(1 << 42) + i * 960) for i in range(6000)]
+    descs += [desc(dst=(1 << 43) + i * 120, pitch=60 * 40, up=(1 << 41) + i * 1600, down=(1 << 42) + i * 960) for i in range(40)]
+    random.Random(1).shuffle(descs)
+    assert need(*descs) == 6040 * 512 * 32 * 2  # (too many tiles to go without packed factors)
+    for bad in (desc(dst=(1 << 40) + 4000 * 12000 + 11998, up=1 << 20, down=1 << 21, rows=1), desc(dst=(1 << 43) + 118, pitch=60 * 40),
+                desc(dst=(1 << 41) + 1600 * 3), desc(dst=1 << 44, src=(1 << 40) + 6000 * 12000 - 2)):
+        assert need(*descs, bad) == INVAL and need(bad, *descs) == INVAL
+
+
+def test_struct_layouts_are_the_headers(tmp_path):
+    """Offsets and sizes of both descriptors as a C compiler lays them out."""
+    import subprocess
+
+    lines = []
+    for struct, cls in (("fstx_low_rank_desc", _native.FstxLowRankDesc), ("fstx_orthogonalize_desc", _native.FstxOrthogonalizeDesc)):
+        lines += [f'_Static_assert(offsetof({struct}, {name}) == {getattr(cls, name).offset}, "{name}");' for name, _ in cls._fields_]
+        lines.append(f'_Static_assert(sizeof({struct}) == {ctypes.sizeof(cls)}, "{struct}");')
+    source = tmp_path / "layout.c"
+    source.write_text('#include <stddef.h>\n#include "fstx_update.h"\n' + "\n".join(lines) + "\n")
+    subprocess.run(["gcc", "-std=c11", "-fsyntax-only", "-I", os.path.join(ROOT, "include"), str(source)], check=True)
+
+
 def test_python_refuses_what_is_not_in_gpu_memory():
     w, u, d = torch.zeros(4, 6), torch.zeros(4, 2), torch.zeros(2, 6)
     with pytest.raises(ValueError, match="GPU memory"):

@@ -279,6 +279,9 @@ def test_refusals(dev):
     refused(RuntimeError, "requires a gradient", w, u.clone().requires_grad_(), d)
     with pytest.raises(ValueError, match="overlap"):
         merge_low_rank([LowRankUpdate(w, u, d), LowRankUpdate(w, u, d)])
+    for scale in (float("inf"), float("nan"), 1e39):
+        refused(ValueError, "finite", w, u, d, scale=scale)
+        refused(ValueError, "finite", w, u, d, scale=scale, out=torch.empty_like(w))
     leaf = u.clone().requires_grad_()
     with torch.no_grad():
         merge_low_rank([LowRankUpdate(w, leaf, d)])
@@ -292,3 +295,15 @@ def test_a_merge_in_place_is_seen_by_autograd(dev):
     merge_low_rank([LowRankUpdate(w, u, d)])
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_from_plain_c():
+    """A C99 program with no Python, torch or C++ in it merges and orthogonalises and checks the results on the host."""
+    import os
+    import subprocess
+
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cabi_update", "cabi_update.bin")
+    if not os.path.exists(exe):
+        pytest.skip("tests/cabi_update/cabi_update.bin is not built (run __graft_entry__.build())")
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and "cabi_update: ok" in run.stdout, run.stdout + run.stderr

@@ -62,12 +62,32 @@ def test_overlaps():
     assert need(desc(dst=BASE, src=BASE, strides=(1, 100))) == INVAL
 
 
+def test_blocks_of_one_tensor_do_not_overlap():
+    left, right = desc(pitch=600, src=BASE, strides=(600, 1)), desc(dst=BASE + 600, src=BASE + 600, pitch=600, strides=(600, 1))
+    assert need(left, right) > 0 and need(right, left) > 0
+    assert need(left, desc(dst=BASE + 598, src=3 * BASE, pitch=600)) == INVAL
+    # an update stored by columns beside the columns that another result is stored in
+    assert need(desc(dst=3 * BASE, src=BASE, strides=(1, 200)), desc(dst=BASE + 200, src=BASE + 200, rows=300, cols=100, pitch=200, strides=(200, 1))) > 0
+    many = [desc(dst=(1 << 40) + i * 60000, src=(1 << 41) + i * 60000) for i in range(6000)]
+    assert need(*many) > 0 and need(*many, desc(dst=(1 << 41) + 6000 * 60000 - 2, src=1 << 20)) == INVAL
+
+
+def test_kinds_of_matrices_beyond_those_kept():
+    """Thirty and more kinds (by the steps that run on shorter operands) in one call plan as each of them alone."""
+    c = (ctypes.c_float * 192)(*[v for _ in range(64) for v in (1.05, 0.1, 0.01)])
+    fn = _native.lib().fstx_orthogonalize_workspace
+    descs = [desc(dst=(1 << 44) + (i << 36), src=(1 << 45) + (i << 36), rows=int(512 * 1.11**i), cols=int(512 * 1.11**i)) for i in range(46)]
+    each = [fn((_native.FstxOrthogonalizeDesc * 1)(d), 1, c, 64) for d in descs]
+    assert fn((_native.FstxOrthogonalizeDesc * 46)(*descs), 46, c, 64) == max(each)
+
+
 def test_steps_eps_and_workspace_are_checked():
     fn, arr, c = _native.lib().fstx_orthogonalize, (_native.FstxOrthogonalizeDesc * 1)(desc()), (ctypes.c_float * 3)(1.5, -0.5, 0.0)
     n = _native.lib().fstx_orthogonalize_workspace(arr, 1, c, 1)
     assert n > 0
     for args in ((arr, 1, c, 0, 0.0, 0x1000, n), (arr, 1, c, 65, 0.0, 0x1000, n), (arr, 1, None, 1, 0.0, 0x1000, n),
-                 (arr, 1, c, 1, -1.0, 0x1000, n), (arr, 1, c, 1, float("nan"), 0x1000, n), (arr, 1, c, 1, 0.0, None, n),
+                 (arr, 1, c, 1, -1.0, 0x1000, n), (arr, 1, c, 1, float("nan"), 0x1000, n), (arr, 1, c, 1, float("inf"), 0x1000, n),
+                 (arr, 1, (ctypes.c_float * 3)(1.0, float("nan"), 0.0), 1, 0.0, 0x1000, n), (arr, 1, c, 1, 0.0, None, n),
                  (arr, 1, c, 1, 0.0, 0x1010, n), (arr, 1, c, 1, 0.0, 0x1000, n - 1), (None, 1, c, 1, 0.0, 0x1000, n)):
         assert fn(*args, None) == INVAL
     assert fn(None, 0, c, 1, 0.0, None, 0, None) == 0
@@ -83,6 +103,8 @@ def test_python_refusals_without_a_gpu():
         orthogonalize([], coefficients=[(1.0, float("inf"), 0.0)])
     with pytest.raises(ValueError, match="finite"):
         orthogonalize([], eps=-1.0)
+    with pytest.raises(ValueError, match="32-bit"):
+        orthogonalize([], coefficients=[(1e39, 0.0, 0.0)])
     with pytest.raises(ValueError, match="outs for"):
         orthogonalize([torch.zeros(3, 4)], outs=[])
     assert orthogonalize([]) == []

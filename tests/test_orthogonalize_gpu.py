@@ -176,6 +176,16 @@ def test_strides_pitch_and_in_place(dev):
     check(x, g, "bf16")
 
 
+def test_column_blocks_of_one_tensor_in_place(dev):
+    """The parts of a fused projection's update, each made orthogonal where it lies."""
+    whole = make(96, 640, 41).to(dev)
+    parts = whole.split([320, 192, 128], dim=1)
+    want = orthogonalize([p.clone() for p in parts])
+    got = orthogonalize(list(parts), outs=list(parts))
+    for g, w, p in zip(got, want, whole.split([320, 192, 128], dim=1)):
+        assert torch.equal(g, w) and torch.equal(p, w)
+
+
 def test_the_result_does_not_depend_on_the_run_and_hardly_on_the_batch(dev):
     """Bit for bit the same from run to run; alone or among others the sums may be split differently, which
     is a difference in their 32-bit rounding only (and a step of the result's type where that decides)."""
