@@ -240,7 +240,9 @@ template <uint32_t left> __device__ __forceinline__ void wait_and_meet() {
 // products, and reads gathered into the first half of a stage changed nothing or cost 1 to 10 %.
 template <uint32_t TR, uint32_t TC, uint32_t Terms> struct Product {
     static constexpr uint32_t kKb = Terms == 1 || TR == 64 ? 2 : 1;                // k blocks per stage
-    static constexpr uint32_t kBufs = 3;                                      // stages in LDS: one computed on, two on their way
+    // Stages in LDS: one computed on, the others on their way.  Small tiles run where few workgroups wait for
+    // each other's results from memory: four, [768, 768] fp32 155 us instead of 182, [1500, 3000] bf16 380 instead of 405 (five: the same).
+    static constexpr uint32_t kBufs = TR == 64 ? 4 : 3;
     static constexpr uint32_t kHalfP = TR / 32 * kKb * Terms;                 // blocks of either operand per stage
     static constexpr uint32_t kHalfQ = TC / 32 * kKb * Terms;
     static constexpr uint32_t kStage = (kHalfP + kHalfQ) * kBlk;              // elements per stage
@@ -385,8 +387,13 @@ __device__ __forceinline__ void store_block(half_t *m, uint64_t plane, uint32_t 
 __device__ __forceinline__ void split(const v16f &v, half_t (&h)[16], half_t (&l)[16]) {
 #pragma unroll
     for (uint32_t r = 0; r < 16; ++r) {
-        h[r] = (half_t)v[r];
-        l[r] = (half_t)(v[r] - (float)h[r]);
+        // One value for both terms: folded into the product before it, as the compiler otherwise may for one of them, the
+        // conversion rounds the unrounded product, now and then to the neighbour of the h that l is the rest of
+        // ([129, 129] fp32 2e-5 off instead of 1.2e-6).
+        float x = v[r];
+        asm("" : "+v"(x));
+        h[r] = (half_t)x;
+        l[r] = (half_t)(x - (float)h[r]);
     }
 }
 
@@ -413,11 +420,6 @@ __global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const
     const uint32_t ji = job_of(t, blockIdx.x);
     const Job job = fetch_job(t, ji);
     const uint32_t lane = threadIdx.x & 63;
-    double sum = 0;
-    for (uint32_t i = lane; i < job.n_partials; i += 64) sum += job.partials[i];
-    const float norm = (float)sqrt(wave_sum(sum));
-    const float factor = job.scale / (norm + eps);
-
     const View g = view_of(job);
     const uint32_t p_blocks = pad_to(job.p, kPadP) / 16, q_blocks = pad_to(job.q, kPadQ) / 16;
     const uint32_t across = (g.x_cols ? q_blocks : p_blocks) / 2, down = (g.x_cols ? p_blocks : q_blocks) / 2;
@@ -429,8 +431,12 @@ __global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const
 #pragma unroll
     for (uint32_t r = 0; r < 16; ++r) {
         const uint32_t row = rb * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-        v[r] = row < g.rows && col < g.cols ? load_elem(job.src, (uint64_t)row * g.row_stride + (uint64_t)col * g.col_stride, job.type) * factor : 0.0f;
+        v[r] = row < g.rows && col < g.cols ? load_elem(job.src, (uint64_t)row * g.row_stride + (uint64_t)col * g.col_stride, job.type) : 0.0f;
     }
+    double sum = 0; // (while the elements are on their way)
+    for (uint32_t i = lane; i < job.n_partials; i += 64) sum += job.partials[i];
+    const float norm = (float)sqrt(wave_sum(sum));
+    v *= job.scale / (norm + eps);
     half_t h[16], l[16], ht[16], lt[16];
     split(v, h, l);
     exchange(h, ht, lane);
@@ -934,8 +940,8 @@ template <uint32_t TR, uint32_t TC, uint32_t Terms> struct Cost;
         static constexpr uint32_t kResident = RESIDENT;                                                              \
         static constexpr double kFixed = FIXED, kShared = SHARED, kAlone = ALONE;                                    \
     };
-FSTX_COST(64, 64, 1, 6, 2.5, 0.057, 0.08)
-FSTX_COST(64, 64, 2, 3, 2.5, 0.12, 0.15)
+FSTX_COST(64, 64, 1, 5, 2.5, 0.057, 0.08)
+FSTX_COST(64, 64, 2, 2, 2.5, 0.12, 0.15)
 FSTX_COST(128, 128, 1, 3, 3.5, 0.165, 0.20)
 FSTX_COST(128, 128, 2, 3, 3.5, 0.355, 0.36)
 FSTX_COST(256, 128, 1, 2, 5.0, 0.275, 0.35)
@@ -1077,7 +1083,7 @@ struct Launcher {
         // entries of X are at most about 1.2 (the spectral norm), their mean square is 1 / (p q) at first
         const double mid = sqrt((double)s.p * (double)s.q);
         j.scale = power_of_two_below(mid < 8192.0 ? mid : 8192.0);
-        const uint64_t parts = (s.p * s.q + 8191) / 8192;
+        const uint64_t parts = (s.p * s.q + 1023) / 1024;
         j.n_partials = (uint32_t)(parts < kPartials ? parts : kPartials);
     }
 };
