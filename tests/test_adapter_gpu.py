@@ -200,3 +200,37 @@ def test_checkpoints_that_do_not_fit_change_nothing(tmp_path):
     assert torch.equal(bufs.get_tensor("a").cpu(), base["a"])
     for x in (bufs, good, l0, l1):
         x.close()
+
+
+def test_checkpoints_then_an_adapter_then_a_rank_s_shards(tmp_path):
+    """Both operators on one loaded file, as a server that specialises a base checkpoint uses them: fine-tuned checkpoints merged in,
+    an adapter merged on top, the adapter taken out again, a rank's block cut -- on a stream of its own, without a synchronisation."""
+    shapes = {"q.weight": (192, 128), "down.weight": (96, 320)}
+    specs = [TensorSpec(n, DType.F32, s) for n, s in shapes.items()]
+    base = write(tmp_path / "base.safetensors", specs, 30)
+    tuned = write(tmp_path / "tuned.safetensors", specs, 31)
+    factors = write(tmp_path / "adapter.safetensors", pair("q", 192, 128, 6, DType.F32) + pair("down", 96, 320, 40, DType.F32), 32)
+    pg = StubProcessGroup(1, 2)
+    (l0, bufs), (l1, other), (l2, adapter) = (load(tmp_path / f"{n}.safetensors", pg=g) for n, g in
+                                              (("base", pg), ("tuned", SingleGroup()), ("adapter", SingleGroup())))
+    bufs.auto_mem_delete = False
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        bufs.merge_checkpoints([other], scale=1.0)
+        bufs.merge_adapter(adapter, scale=2.0)
+        with_adapter = {n: bufs.get_sharded(n, 0).clone() for n in shapes}
+        bufs.merge_adapter(adapter, scale=-2.0)
+        without = {n: bufs.get_sharded(n, 1).clone() for n in shapes}
+    stream.synchronize()
+    for n, (rows, cols) in shapes.items():
+        w = base[n].double()
+        o, s = polar(tuned[n].double() - w)
+        a, b = (factors[f"{PREFIX}{n[:-7]}.lora_{k}.weight"].double() for k in "AB")
+        merged, r = w + s * o, a.shape[0]
+        # the orthogonal part as in the test above; each merge adds its own 32-bit roundings (six products per k, see close())
+        slack = 1e-3 * s + (2 * (b.abs() @ a.abs()) * ((6 * r + 4) * 2.0**-23) + 2.0**-22 * (merged.abs() + 2 * (b @ a).abs())) * 2
+        want, half = merged + 2 * (b @ a), rows // 2
+        assert ((with_adapter[n].cpu().double() - want[half:]).abs() <= slack[half:]).all(), n
+        assert ((without[n].cpu().double() - merged[:, cols // 2 :]).abs() <= slack[:, cols // 2 :]).all(), n
+    for x in (bufs, other, adapter, l0, l1, l2):
+        x.close()
