@@ -109,11 +109,24 @@ __device__ __forceinline__ uint32_t column_of(uint32_t blk, uint32_t rho, uint32
     return 4 * per * v + per * (rho >> 2) + 4 * tt + (rho & 3);
 }
 
-__device__ __forceinline__ float load_factor(const char *src, uint64_t at, uint32_t type) {
-    if (type == FSTX_F32) return *(const FSTX_GLOBAL float *)(src + at * 4);
-    const uint16_t raw = *(const FSTX_GLOBAL uint16_t *)(src + at * 2);
-    if (type == FSTX_BF16) return __builtin_bit_cast(float, (uint32_t)raw << 16);
-    return (float)__builtin_bit_cast(_Float16, raw);
+// Eight elements of a factor, those at(e) that are there(e), zeros else.  All eight loads go out together: the type is
+// looked at once, and what is not there is read from the factor's first element and dropped, where a branch around each load
+// would wait for one after the other (the merge of a Llama-3-8B layer 182.7 us instead of 185.1).
+template <typename At, typename There>
+__device__ __forceinline__ void load_factor(const char *src, uint32_t type, float (&x)[8], At at, There there) {
+    if (type == FSTX_F32) {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) x[e] = *(const FSTX_GLOBAL float *)(src + (there(e) ? at(e) : 0) * 4);
+    } else {
+        uint16_t raw[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) raw[e] = *(const FSTX_GLOBAL uint16_t *)(src + (there(e) ? at(e) : 0) * 2);
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e)
+            x[e] = type == FSTX_BF16 ? __builtin_bit_cast(float, (uint32_t)raw[e] << 16) : (float)__builtin_bit_cast(_Float16, raw[e]);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) x[e] = there(e) ? x[e] : 0.0f;
 }
 
 // the bf16 nearest to x; where that would overflow a finite x, the one below it
@@ -151,10 +164,8 @@ __global__ __launch_bounds__(256) void pack_factors_kernel(const Jobs<PackJob> t
     const uint32_t row = job.per ? column_of(blk, rho, job.per) : blk * 16 + rho;
     const uint32_t k0 = kb * kK + 8 * (lane >> 4);
     float x[8];
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e)
-        x[e] = row < job.rows && k0 + e < job.rank
-                   ? load_factor(job.src, (uint64_t)row * job.row_stride + (uint64_t)(k0 + e) * job.k_stride, job.type) : 0.0f;
+    load_factor(job.src, job.type, x, [&](uint32_t e) { return (uint64_t)row * job.row_stride + (uint64_t)(k0 + e) * job.k_stride; },
+                [&](uint32_t e) { return row < job.rows && k0 + e < job.rank; });
     uint16_t *out = job.dst + ((uint64_t)lb * job.terms) * kBlk + lane * 8;
     if (job.half) {
         *(FSTX_GLOBAL v8h *)out = half_terms(x);
@@ -550,10 +561,10 @@ template <uint32_t T, uint32_t Cls> __global__ __launch_bounds__(256) void direc
         const uint64_t row_stride = cols ? job.down_col : job.up_row, k_stride = cols ? job.down_k : job.up_k;
         const uint32_t type = cols ? job.down_type : job.up_type;
         const bool live = row < (cols ? m.cols : m.rows);
-        float x[8];
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e)
-            x[e] = live && k0 + e < job.rank ? load_factor(src, (uint64_t)row * row_stride + (uint64_t)(k0 + e) * k_stride, type) : 0.0f;
+        float x[8] = {};
+        if (job.rank)
+            load_factor(src, type, x, [&](uint32_t e) { return (uint64_t)row * row_stride + (uint64_t)(k0 + e) * k_stride; },
+                        [&](uint32_t e) { return live && k0 + e < job.rank; });
         uint16_t *out = lds + b * kTerms * kBlk + lane * 8;
         if constexpr (Cls == kTermsH1) *(v8h *)out = half_terms(x);
         else
