@@ -17,7 +17,7 @@
 //                        No LDS and no barriers: nothing is shared but the factors.
 //
 // What bounds it, measured.  The seven matrices of a Llama-3-8B layer, bf16, rank 64 (883 MB read and written):
-// 169 us + 15 us of packing, 5.2 TB/s; a plain copy of that size does 6.2.  A Llama-3-70B fp8 layer, rank 16
+// 169 us + 14 us of packing, 5.2 TB/s; a plain copy of that size does 6.2.  A Llama-3-70B fp8 layer, rank 16
 // (1.7 GB): 360 us, 4.8 TB/s.  Steps there (same layer): one 64 x 64 tile per wavefront with 64 contiguous bytes per row and
 // instruction 241 us, 26 % more written to HBM than the weight holds, because half lines left L2 before their other
 // halves came; whole lines per instruction 193 us; walks of four tiles 184 (of eight 189, of two 180 but 364 instead of
