@@ -25,8 +25,8 @@ extern "C" {
  * Products and sums are held in 32 bits; factors of f32 are split into bf16 terms, as many as the
  * weight's type can tell apart.  With FSTX_F8_E4M3 weights W stands for W * weight_scale[row] and the
  * result is (W * weight_scale + scale * up @ down) / weight_scale, saturated to +-448 (a NaN stays one).
- * An infinity in a factor makes its row or column infinite or NaN.  Up to 2^31 - 256 rows and columns and about
- * 6 * 10^9 elements (-FSTX_E_RANGE). */
+ * An infinity in a factor makes its row or column infinite or NaN.  Up to about
+ * 6 * 10^9 elements, and 10^8 rows and columns together per 32 of the rank (-FSTX_E_RANGE). */
 typedef struct fstx_low_rank_desc {
     void *dst;                  /* [rows, cols] elements of `type`, rows dst_pitch elements apart       */
     const void *src;            /* [rows, cols] elements of `type`, rows src_pitch elements apart       */
