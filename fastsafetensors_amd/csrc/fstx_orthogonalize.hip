@@ -466,11 +466,12 @@ __global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const
                    [&](uint32_t r) { return row_of(r) < g.rows && col < g.cols; });
     double sum = 0; // (while the elements are on their way)
     for (uint32_t i = lane; i < job.n_partials; i += 64) sum += job.partials[i];
-    const float norm = (float)sqrt(wave_sum(sum));
-    const float factor = job.scale / (norm + eps);
+    // 1 / (|G| + eps) may lie outside of what 32 bits hold, its mantissa and exponent do not
+    int exponent;
+    const float factor = (float)((double)job.scale / frexp(sqrt(wave_sum(sum)) + (double)eps, &exponent));
     v16f v;
 #pragma unroll
-    for (uint32_t r = 0; r < 16; ++r) v[r] = x[r] * factor;
+    for (uint32_t r = 0; r < 16; ++r) v[r] = __builtin_ldexpf(x[r], -exponent) * factor;
     half_t h[16], l[16], ht[16], lt[16];
     split(v, h, l);
     exchange(h, ht, lane);

@@ -59,7 +59,8 @@ int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, void *works
  * held in 22 bits and products as accurate as 32-bit ones, shorter operands only where a result of the
  * type cannot tell; sums are held in 32 bits, the norm's in 64.  While the steps run the
  * iterates' singular values have to stay below about 2 (those of X start at 1 or less).  With up to 32 rows
- * or columns everything is done in 64 bits.  An infinity or a NaN anywhere makes the whole result NaN. */
+ * or columns everything is done in 64 bits.  Infinities and NaN spread through the result
+ * as they do in the formula. */
 typedef struct fstx_orthogonalize_desc {
     void *dst;                              /* [rows, cols] of `type`, rows dst_pitch elements apart     */
     const void *src;                        /* [rows, cols] of `type`, any strides (elements); dst or apart */

@@ -127,6 +127,14 @@ def test_scales_of_the_input(dev):
     check(orthogonalize(g.to(dev), eps=0.5), g, "f32", eps=0.5, core=1e-4)  # eps of the norm's size: small singular values
 
 
+def test_norms_that_32_bits_do_not_hold(dev):
+    g = make(40, 90, 3, scale=1.0)
+    for scale in (2.0**125, 2.0**-130):  # |G| is 2.5e39; and elements of a few denormal digits
+        x = g * scale
+        assert x.isfinite().all()
+        check(orthogonalize(x.to(dev), eps=0.0), x, "f32", eps=0.0)
+
+
 def test_zero_matrix_and_special_values(dev):
     assert (orthogonalize(torch.zeros(50, 70, device=dev)) == 0).all()
     for bad in (float("nan"), float("inf")):
@@ -174,6 +182,67 @@ def test_strides_pitch_and_in_place(dev):
     x = g.to(dev)
     assert orthogonalize(x, outs=x) is x
     check(x, g, "bf16")
+
+
+def slim_close(got, g, coefficients=FIVE):
+    want = iterate(g, coefficients)  # 64 bits on both sides: half a step of the type, as in test_slim_matrices
+    return ((got.cpu().double() - want).abs() <= want.abs() * (torch.finfo(g.dtype).eps / 2 * 1.001) + 2.0**-25 + want.abs().max() * 2.0**-40).all()
+
+
+def test_more_slim_matrices_than_one_set_takes(dev):
+    """Seventy of them between larger and empty ones: every second stored by columns, some pitched, all in place."""
+    mats, kept = [], []
+    for i in range(70):
+        m, n, t = 1 + i * 5 % 32, 1 + i * 37 % 300, list(T)[i % 3]
+        g = make(m, n, i).to(T[t]) if i % 4 < 2 else make(n, m, i).to(T[t])
+        kept.append(g)
+        held = torch.full((g.shape[0], g.shape[1] + i % 3), 7.0, dtype=g.dtype, device=dev)
+        at = held[:, : g.shape[1]] if i % 2 else torch.empty(g.shape[::-1], dtype=g.dtype, device=dev).t()
+        at.copy_(g)
+        mats.append(at)
+        if i % 20 == 0:
+            mats += [torch.empty(0, 5, device=dev), make(100, 90, i).to(dev)]
+            kept += [None, None]
+    out = orthogonalize(mats, outs=mats)
+    for at, g, o in zip(mats, kept, out):
+        assert o is at and (g is None or slim_close(at, g)), at.shape
+    held = torch.full((8, 40), 7.0, device=dev)
+    orthogonalize([held[:, :33].copy_(make(8, 33))], outs=[held[:, :33]])
+    assert (held[:, 33:] == 7.0).all()  # what lies between the rows stays
+
+
+def test_special_values_in_slim_matrices(dev):
+    g = make(12, 100, 5)
+    assert torch.equal(orthogonalize(torch.zeros(12, 100, device=dev)).cpu(), torch.zeros(12, 100))
+    assert orthogonalize(torch.zeros(12, 100, device=dev), eps=0.0).isnan().all()
+    for bad in (float("inf"), float("nan")):
+        b = g.clone()
+        b[3, 77] = bad
+        got = orthogonalize([b.to(dev), g.to(dev)])
+        assert got[0].isnan().all() and slim_close(got[1], g)
+    # squares of the largest floats do not overflow, nor do those of small ones vanish
+    for scale in (2.0**124, 2.0**-100):
+        got = orthogonalize((g * scale).to(dev), eps=0.0)
+        assert ((got.cpu().double() - iterate(g, eps=0.0)).abs() <= 2.0**-24).all()
+
+
+def test_slim_matrices_captured_and_replayed(dev):
+    g = [make(32, 5000, 1).to(dev), make(900, 7, 2).to(dev)]
+    out = [torch.empty_like(x) for x in g]
+    orthogonalize(g, outs=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        orthogonalize(g, outs=out)
+    for turn in range(3):
+        for i, x in enumerate(g):
+            x.copy_(make(*x.shape, 10 * turn + i))
+        want = orthogonalize(g)
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(out, want))
 
 
 def test_column_blocks_of_one_tensor_in_place(dev):
