@@ -176,8 +176,8 @@ def _launch_low_rank(descs: Any, first: int, n: int, device: torch.device, need:
         _launch_low_rank(descs, first, n // 2, device, -1, stream)
         _launch_low_rank(descs, first + n // 2, n - n // 2, device, -1, stream)
         return
-    space = torch.empty(need, dtype=torch.uint8, device=device)
-    _native.merge_low_rank(at, n, space.data_ptr() if need else 0, need, stream)
+    space = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _native.merge_low_rank(at, n, 0 if space is None else space.data_ptr(), need, stream)
 
 
 def _on_device(device: torch.device) -> Any:
