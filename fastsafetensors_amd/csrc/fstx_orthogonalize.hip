@@ -17,8 +17,12 @@
 // the ten times of fp32 MFMA.  One term is not enough: the iteration multiplies small singular values by a
 // each step, and with them the rounding errors of the first steps, up to a^steps = 485 times;
 // with a few strong directions over a floor of weak ones a single fp16 term ends 2 to 3 % off (bf16:
-// 20 %), measured on spectra with a ratio of 1000.  What has to keep both terms is X itself, in a X; whether the
-// products of a step need them depends on how large B X is beside a X, see one_term_steps.
+// 20 %), measured on spectra with a ratio of 1000.  Nor is it enough in the first steps alone, where B X is small beside
+// a X if all singular values are small: where one row holds most of an update, one of them is near 1 from the start and B
+// all but a single element, whose rounding nothing averages ([2560, 2560] fp32 1.5e-3 off, [768, 768] bf16 3.3e-3 instead of
+// 1.6e-3).  The host, which launches the steps, does not see the spectrum: all products are of two terms, for
+// results of every type.  (With one term in three or four of five steps [14336, 4096] bf16 took 5.4 ms instead of 10.2, [1024, 4096] bf16 265 us
+// instead of 367.)
 // fp16 rather than bf16 terms because the iterates are bounded: entries of X are at most about
 // 1.2, they are held times a power of two near sqrt(p q) so that their typical size stays in the
 // middle of fp16's range; A and B are held times fixed powers of two likewise.
@@ -55,6 +59,7 @@ typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 half_t;
 
 constexpr uint32_t kBlk = 512;        // elements of one block (32 rows x 16 k) of one term
+constexpr uint32_t kTerms = 2;
 constexpr uint32_t kPadP = 256, kPadQ = 256; // sides are stored padded to these (the largest tile)
 constexpr uint32_t kStepPad = 64;            // ... and summed over padded to this
 constexpr uint32_t kMaxJobs = 20;
@@ -262,22 +267,20 @@ template <uint32_t left> __device__ __forceinline__ void wait_and_meet() {
 // multiplied from registers the next one is read from LDS into other registers and two more are on
 // their way from memory to LDS; reads and loads are issued in between the products.
 //
-// What bounds it.  B X of a [14336, 4096] update, 0.48 * 10^15 operations in fp16: two terms (three products) 1.07 to
+// What bounds it.  B X of a [14336, 4096] update, three products of 0.48 * 10^12 operations each in fp16: 1.07 to
 // 1.2 ms with 256 x 256 tiles, 1.2 to 1.35 PFLOP/s; the library's 8192^3 fp16 product does 1.3 to 1.5 on the same cards
 // with the matrix cores busy 94 % of the time at 1.43 GHz -- the power limit -- and this one 80 % at 1.6 GHz.
-// One term takes 0.46 to 0.49 ms, 1.0 PFLOP/s: with the products of a step down to a third, the 600 MB that
-// the ends of the tiles read and write (X in two terms, X^T) take 0.12 ms of their own, only part of which another
-// workgroup on the compute unit hides.  Steps on the way, same product in two terms: 1.45 ms with 128 x 128 tiles, 32 k per
+// Steps on the way, same product: 1.45 ms with 128 x 128 tiles, 32 k per
 // stage and one stage ahead; 1.3 with 16 k and two ahead; 1.15 with 256 x 128 tiles; 1.07 with 256 x 256, reads between the
 // products and the ends' loads put before their stores.  More stages ahead, raised wave priority around the
 // products, and reads gathered into the first half of a stage changed nothing or cost 1 to 10 %.
-template <uint32_t TR, uint32_t TC, uint32_t Terms> struct Product {
-    static constexpr uint32_t kKb = Terms == 1 || TR == 64 ? 2 : 1;                // k blocks per stage
+template <uint32_t TR, uint32_t TC> struct Product {
+    static constexpr uint32_t kKb = TR == 64 ? 2 : 1;                         // k blocks per stage
     // Stages in LDS: one computed on, the others on their way.  Small tiles run where few workgroups wait for
     // each other's results from memory: four, [768, 768] fp32 155 us instead of 182, [1500, 3000] bf16 380 instead of 405 (five: the same).
     static constexpr uint32_t kBufs = TR == 64 ? 4 : 3;
-    static constexpr uint32_t kHalfP = TR / 32 * kKb * Terms;                 // blocks of either operand per stage
-    static constexpr uint32_t kHalfQ = TC / 32 * kKb * Terms;
+    static constexpr uint32_t kHalfP = TR / 32 * kKb * kTerms;                 // blocks of either operand per stage
+    static constexpr uint32_t kHalfQ = TC / 32 * kKb * kTerms;
     static constexpr uint32_t kStage = (kHalfP + kHalfQ) * kBlk;              // elements per stage
     static constexpr uint32_t kLoads = (kHalfP + kHalfQ) / 4;                 // per wavefront and stage
     static constexpr uint32_t kWaves = TR * TC > 256 * 128 ? 1 : 2;           // wavefronts per SIMD the registers are divided for
@@ -295,8 +298,8 @@ template <uint32_t TR, uint32_t TC, uint32_t Terms> struct Product {
             const uint32_t at = n * 4 + wave;
             const bool second = n * 4 >= kHalfP;
             const uint32_t in = second ? at - kHalfP : at;
-            const uint32_t rb = in / (kKb * Terms), rest = in % (kKb * Terms);
-            const half_t *from = (second ? q : p) + rb * row_step + (uint64_t)(kb0 + rest / Terms) * kBlk + (rest % Terms ? pick(second, q_plane, p_plane) : 0) + lane * 8;
+            const uint32_t rb = in / (kKb * kTerms), rest = in % (kKb * kTerms);
+            const half_t *from = (second ? q : p) + rb * row_step + (uint64_t)(kb0 + rest / kTerms) * kBlk + (rest % kTerms ? pick(second, q_plane, p_plane) : 0) + lane * 8;
             __builtin_amdgcn_global_load_lds((const FSTX_GLOBAL void *)from, (FSTX_LDS void *)(lds + buf * kStage + at * kBlk), 16, 0, 0);
         };
         auto load_stage = [&](uint32_t kb0, uint32_t buf) {
@@ -304,14 +307,14 @@ template <uint32_t TR, uint32_t TC, uint32_t Terms> struct Product {
             for (uint32_t n = 0; n < kLoads; ++n) load_part(kb0, buf, n);
         };
         struct Fragments {
-            v8h p[kKb][kNR][Terms], q[kKb][kNC][Terms];
+            v8h p[kKb][kNR][kTerms], q[kKb][kNC][kTerms];
         };
         // A stage's LDS reads and its products, numbered: reads in the order in which products want them
-        constexpr uint32_t kReads = kKb * Terms * (kNR + kNC), kPerKb = (Terms == 1 ? 1 : 3) * kNR * kNC, kProducts = kKb * kPerKb;
+        constexpr uint32_t kReads = kKb * kTerms * (kNR + kNC), kPerKb = 3 * kNR * kNC, kProducts = kKb * kPerKb;
         auto read = [&](const half_t *base, Fragments &f, uint32_t r) {
-            const uint32_t kb = r / (Terms * (kNR + kNC)), m = r / (kNR + kNC) % Terms, i = r % (kNR + kNC);
-            if (i < kNR) f.p[kb][i][m] = *(const v8h *)(base + (((wr * kNR + i) * kKb + kb) * Terms + m) * kBlk);
-            else f.q[kb][i - kNR][m] = *(const v8h *)(base + (kHalfP + ((wc * kNC + i - kNR) * kKb + kb) * Terms + m) * kBlk);
+            const uint32_t kb = r / (kTerms * (kNR + kNC)), m = r / (kNR + kNC) % kTerms, i = r % (kNR + kNC);
+            if (i < kNR) f.p[kb][i][m] = *(const v8h *)(base + (((wr * kNR + i) * kKb + kb) * kTerms + m) * kBlk);
+            else f.q[kb][i - kNR][m] = *(const v8h *)(base + (kHalfP + ((wc * kNC + i - kNR) * kKb + kb) * kTerms + m) * kBlk);
         };
         auto product = [&](const Fragments &f, uint32_t n) {
             const uint32_t kb = n / kPerKb, kind = n % kPerKb / (kNR * kNC), i = n / kNC % kNR, j = n % kNC;
@@ -383,14 +386,13 @@ __device__ __forceinline__ uint64_t quad_at(uint32_t rb, uint32_t cb, uint32_t k
 struct RawBlock {
     v4h h[4], l[4];
 };
-__device__ __forceinline__ RawBlock load_block(const half_t *m, uint64_t plane, uint32_t rb, uint32_t cb, uint32_t k_blocks_stored, uint32_t lane, bool both) {
+__device__ __forceinline__ RawBlock load_block(const half_t *m, uint64_t plane, uint32_t rb, uint32_t cb, uint32_t k_blocks_stored, uint32_t lane) {
     RawBlock out;
 #pragma unroll
     for (uint32_t g = 0; g < 4; ++g) {
         const half_t *at = m + quad_at(rb, cb, k_blocks_stored, g, lane);
         out.h[g] = *(const FSTX_GLOBAL v4h *)at;
-        out.l[g] = v4h{};
-        if (both) out.l[g] = *(const FSTX_GLOBAL v4h *)(at + plane);
+        out.l[g] = *(const FSTX_GLOBAL v4h *)(at + plane);
     }
     return out;
 }
@@ -402,7 +404,7 @@ __device__ __forceinline__ v16f value_of(const RawBlock &b) {
 }
 
 __device__ __forceinline__ void store_block(half_t *m, uint64_t plane, uint32_t rb, uint32_t cb, uint32_t k_blocks_stored, uint32_t lane, const half_t (&h)[16],
-                                            const half_t (&l)[16], bool both) {
+                                            const half_t (&l)[16]) {
 #pragma unroll
     for (uint32_t g = 0; g < 4; ++g) {
         half_t *at = m + quad_at(rb, cb, k_blocks_stored, g, lane);
@@ -413,7 +415,7 @@ __device__ __forceinline__ void store_block(half_t *m, uint64_t plane, uint32_t 
             vl[e] = l[4 * g + e];
         }
         *(FSTX_GLOBAL v4h *)at = vh;
-        if (both) *(FSTX_GLOBAL v4h *)(at + plane) = vl;
+        *(FSTX_GLOBAL v4h *)(at + plane) = vl;
     }
 }
 
@@ -449,7 +451,7 @@ __device__ __forceinline__ void exchange(const half_t (&in)[16], half_t (&out)[1
 }
 
 // X and X^T from G: a wavefront takes a 32 x 32 block, its lanes along the side along which memory runs.
-__global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const float eps, const uint32_t low_term) {
+__global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const float eps) {
     const uint32_t ji = job_of(t, blockIdx.x);
     const Job job = fetch_job(t, ji);
     const uint32_t lane = threadIdx.x & 63;
@@ -477,13 +479,12 @@ __global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const
     exchange(h, ht, lane);
     exchange(l, lt, lane);
     const uint64_t plane = plane_of(p_blocks, q_blocks);
-    // X's second term is always wanted (a X keeps both), X^T's where the first product has two terms
     if (g.x_cols) {
-        store_block(job.xt0, plane, cb, rb, p_blocks, lane, h, l, low_term);
-        store_block(job.x, plane, rb, cb, q_blocks, lane, ht, lt, true);
+        store_block(job.xt0, plane, cb, rb, p_blocks, lane, h, l);
+        store_block(job.x, plane, rb, cb, q_blocks, lane, ht, lt);
     } else {
-        store_block(job.x, plane, cb, rb, q_blocks, lane, h, l, true);
-        store_block(job.xt0, plane, rb, cb, p_blocks, lane, ht, lt, low_term);
+        store_block(job.x, plane, cb, rb, q_blocks, lane, h, l);
+        store_block(job.xt0, plane, rb, cb, p_blocks, lane, ht, lt);
     }
 }
 
@@ -492,8 +493,6 @@ enum Phase : uint32_t { kGram, kPoly, kApply, kLast };
 struct Coefficients {
     float own, product;  // result = own * (what is there) + product * (sum of the products)
     uint32_t current;    // which of xt0, xt1 is the current one
-    uint32_t own_both;   // "what is there" is taken with both its terms
-    uint32_t next_both;  // the next step's products want both terms of X^T
 };
 
 // Tiles of a symmetric matrix that reach on or below the diagonal, row by row: row i has kAspect (i + 1) of
@@ -527,16 +526,16 @@ __device__ __forceinline__ RawBlock own_block(const Job &job, const Coefficients
     } else if constexpr (kPhase == kLast) {
         const bool flipped = job.flipped;
         return load_block(pick<const half_t *>(flipped, job.x, pick(c.current, job.xt1, job.xt0)), plane_of(p_blocks, q_blocks), pick(flipped, rb, cb), pick(flipped, cb, rb),
-                          pick(flipped, q_blocks, p_blocks), lane, c.own_both);
+                          pick(flipped, q_blocks, p_blocks), lane);
     } else {
         return load_block(kPhase == kPoly ? job.a : job.x, plane_of(p_blocks, kPhase == kPoly ? p_blocks : q_blocks), rb, cb,
-                          kPhase == kPoly ? p_blocks : q_blocks, lane, c.own_both);
+                          kPhase == kPoly ? p_blocks : q_blocks, lane);
     }
 }
 
 // What becomes of one 32 x 32 block of a product. `v` is laid out with lanes along rows (the transposed
 // product), in the last step of a matrix that is not flipped with lanes along columns.
-template <uint32_t kPhase, uint32_t Terms>
+template <uint32_t kPhase>
 __device__ __forceinline__ void finish_block(const Job &job, const Coefficients &c, uint32_t rb, uint32_t cb, v16f v, const RawBlock &there, uint32_t lane) {
     const uint32_t p_blocks = pad_to(job.p, kPadP) / 16, q_blocks = pad_to(job.q, kPadQ) / 16;
     if constexpr (kPhase == kLast) {
@@ -563,12 +562,11 @@ __device__ __forceinline__ void finish_block(const Job &job, const Coefficients 
         split(v, h, l);
         half_t *to = kPhase == kGram ? job.a : kPhase == kPoly ? job.b : job.x;
         const uint64_t plane = plane_of(p_blocks, kPhase == kApply ? q_blocks : p_blocks);
-        store_block(to, plane, rb, cb, kPhase == kApply ? q_blocks : p_blocks, lane, h, l, kPhase == kApply || Terms == 2);
+        store_block(to, plane, rb, cb, kPhase == kApply ? q_blocks : p_blocks, lane, h, l);
         if (kPhase == kApply || cb != rb) {
-            const bool both = kPhase == kApply ? c.next_both : Terms == 2;
             exchange(h, ht, lane);
-            if (both) exchange(l, lt, lane);
-            store_block(kPhase == kApply ? pick(c.current, job.xt0, job.xt1) : to, plane, cb, rb, p_blocks, lane, ht, lt, both);
+            exchange(l, lt, lane);
+            store_block(kPhase == kApply ? pick(c.current, job.xt0, job.xt1) : to, plane, cb, rb, p_blocks, lane, ht, lt);
         }
     }
 }
@@ -593,9 +591,9 @@ __device__ __forceinline__ void place_of(const Job &job, uint32_t tile, uint32_t
     }
 }
 
-template <uint32_t kPhase, uint32_t TR, uint32_t TC, uint32_t Terms>
-__global__ __launch_bounds__(256, (Product<TR, TC, Terms>::kWaves)) void newton_schulz_kernel(const Jobs t, const Deal deal, const Coefficients c) {
-    typedef Product<TR, TC, Terms> Prod;
+template <uint32_t kPhase, uint32_t TR, uint32_t TC>
+__global__ __launch_bounds__(256, (Product<TR, TC>::kWaves)) void newton_schulz_kernel(const Jobs t, const Deal deal, const Coefficients c) {
+    typedef Product<TR, TC> Prod;
     constexpr uint32_t kNR = Prod::kNR, kNC = Prod::kNC;
     __shared__ __attribute__((aligned(1024))) half_t lds[Prod::kBufs * Prod::kStage];
     const uint32_t ji = job_of(t, blockIdx.x);
@@ -660,14 +658,14 @@ __global__ __launch_bounds__(256, (Product<TR, TC, Terms>::kWaves)) void newton_
 #pragma unroll
         for (uint32_t j = 0; j < kNC; ++j)
             if (!symmetric<kPhase>() || cb0 + j <= rb0 + i) // above the diagonal: written as the mirror of (cb, rb)
-                finish_block<kPhase, Terms>(job, c, rb0 + i, cb0 + j, acc[i][j], there[i % 2][j], lane);
+                finish_block<kPhase>(job, c, rb0 + i, cb0 + j, acc[i][j], there[i % 2][j], lane);
     }
 }
 
 // The tiles whose sums came in pieces: a wavefront per 32 x 32 block adds them in order.
-template <uint32_t kPhase, uint32_t TR, uint32_t TC, uint32_t Terms>
+template <uint32_t kPhase, uint32_t TR, uint32_t TC>
 __global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Deal deal, const Coefficients c) {
-    typedef Product<TR, TC, Terms> Prod;
+    typedef Product<TR, TC> Prod;
     constexpr uint32_t kBlocks = TR / 32 * (TC / 32);
     const uint32_t ji = job_of(t, blockIdx.x);
     const Job job = fetch_job(t, ji);
@@ -689,7 +687,7 @@ __global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Dea
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) v[4 * g + e] += part[e];
         }
-    finish_block<kPhase, Terms>(job, c, rb, cb, v, there, threadIdx.x);
+    finish_block<kPhase>(job, c, rb, cb, v, there, threadIdx.x);
 }
 
 // ------------------------------------------------------------ slim matrices
@@ -924,53 +922,20 @@ int check(const fstx_orthogonalize_desc *descs, uint32_t n) {
     return 0;
 }
 
-// Below kOneTermFrom a product's time is the latency of its few stages whatever their number of products: small matrices
-// keep two terms throughout, and matrices of all types share their launches ([1023, 257] and three smaller fp16 ones: 250 us
-// in two sets of launches, 160 in one).
-constexpr uint64_t kOneTermFrom = 512;
-
-// Which steps' products run on one term (bit k: step k).
-//
-// In the first steps a X is nearly all of the result: the singular values s of a matrix whose mean square
-// is 1 / p are small, and B X = (b s^2 + c s^4) X with them.  One term in the products of such a step, with both terms of X
-// in a X, is off by 2^-12 (|b| s^2 + |c| s^4) of the result, s^2 growing by a^2 per step; that model was met within
-// a factor of two on flat, decaying and spiked spectra (64-bit simulation with rounded operands).  A step takes one term
-// where it stays under 2^-12 for bf16 results (2^-9 of rounding), 2^-15 for fp16 (2^-12), 2^-21 for f32
-// (where 32-bit products themselves end at 2^-19 to 2^-17 on spiked spectra).
-// The LAST step of bf16 results takes one term too, in a X as well, so that the rounding of X enters with the slope of
-// the polynomial (below one there) and not with a and B separately: 4e-4 to 7e-4, against 1.7e-3 of rounding.
-uint64_t one_term_steps(const fstx_orthogonalize_desc &d, const float *coefficients, uint32_t steps) {
-    if ((d.rows < d.cols ? d.rows : d.cols) < kOneTermFrom) return 0;
-    const double budget = d.type == FSTX_BF16 ? 0x1p-12 : d.type == FSTX_F16 ? 0x1p-15 : 0x1p-21;
-    double s2 = 1.0 / (double)(d.rows < d.cols ? d.rows : d.cols);
-    uint64_t mask = 0;
-    for (uint32_t k = 0; k < steps; ++k) {
-        const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
-        if (0x1p-12 * (fabs(b) * s2 + fabs(c) * s2 * s2) <= budget && k + 1 < steps) mask |= 1ull << k;
-        s2 = s2 * a * a < 1.0 ? s2 * a * a : 1.0;
-    }
-    if (d.type == FSTX_BF16) mask |= 1ull << (steps - 1);
-    return mask;
-}
-
 inline float power_of_two_below(double v) { return (float)ldexp(1.0, (int)floor(log2(v))); }
 
 // What the tile sizes cost, measured (microseconds): a launch and the ends of a workgroup; 16 k of one workgroup when
 // kResident share a compute unit, per workgroup, and when it is alone there.
-template <uint32_t TR, uint32_t TC, uint32_t Terms> struct Cost;
-#define FSTX_COST(TR, TC, TERMS, RESIDENT, FIXED, SHARED, ALONE)                                                     \
-    template <> struct Cost<TR, TC, TERMS> {                                                                         \
+template <uint32_t TR, uint32_t TC> struct Cost;
+#define FSTX_COST(TR, TC, RESIDENT, FIXED, SHARED, ALONE)                                                     \
+    template <> struct Cost<TR, TC> {                                                                         \
         static constexpr uint32_t kResident = RESIDENT;                                                              \
         static constexpr double kFixed = FIXED, kShared = SHARED, kAlone = ALONE;                                    \
     };
-FSTX_COST(64, 64, 1, 5, 2.5, 0.057, 0.08)
-FSTX_COST(64, 64, 2, 2, 2.5, 0.12, 0.15)
-FSTX_COST(128, 128, 1, 3, 3.5, 0.165, 0.20)
-FSTX_COST(128, 128, 2, 3, 3.5, 0.355, 0.36)
-FSTX_COST(256, 128, 1, 2, 5.0, 0.275, 0.35)
-FSTX_COST(256, 128, 2, 2, 5.0, 0.630, 0.70)
-FSTX_COST(256, 256, 1, 1, 8.0, 0.545, 0.545)
-FSTX_COST(256, 256, 2, 1, 8.0, 1.230, 1.230)
+FSTX_COST(64, 64, 2, 2.5, 0.12, 0.15)
+FSTX_COST(128, 128, 3, 3.5, 0.355, 0.36)
+FSTX_COST(256, 128, 2, 5.0, 0.630, 0.70)
+FSTX_COST(256, 256, 1, 8.0, 1.230, 1.230)
 #undef FSTX_COST
 
 struct Launcher {
@@ -986,8 +951,8 @@ struct Launcher {
     // Deals the tiles to workgroups.  Whole rounds take a tile each.  Tiles that are left over would keep a few compute
     // units busy for the time of a whole tile while the others idle: they can be cut along k into pieces instead, as many
     // as there is room for, at the price of a second launch that joins them.  Returns an estimate in microseconds.
-    template <uint32_t kPhase, uint32_t TR, uint32_t TC, uint32_t Terms> double deal() {
-        typedef Cost<TR, TC, Terms> cost;
+    template <uint32_t kPhase, uint32_t TR, uint32_t TC> double deal() {
+        typedef Cost<TR, TC> cost;
         uint64_t tiles = 0;
         uint32_t blocks = ~0u, longest = 0; // of 16 k
         for (uint32_t i = 0; i < n; ++i) {
@@ -1034,8 +999,8 @@ struct Launcher {
         return best;
     }
 
-    template <uint32_t kPhase, uint32_t TR, uint32_t TC, uint32_t Terms> int launch(const Coefficients &c) {
-        deal<kPhase, TR, TC, Terms>();
+    template <uint32_t kPhase, uint32_t TR, uint32_t TC> int launch(const Coefficients &c) {
+        deal<kPhase, TR, TC>();
         if (!run) {
             const uint64_t bytes = sum_tiles * TR * TC * sizeof(float);
             if (bytes > sum_bytes) sum_bytes = bytes;
@@ -1043,7 +1008,7 @@ struct Launcher {
         }
         {
             fstx_internal::Range range("fstx newton_schulz_kernel: phase %u, %u matrices, %u workgroups, tiles of %u x %u", kPhase, n, grid, TR, TC);
-            hipLaunchKernelGGL((newton_schulz_kernel<kPhase, TR, TC, Terms>), dim3(grid), dim3(256), 0, stream, t, d, c);
+            hipLaunchKernelGGL((newton_schulz_kernel<kPhase, TR, TC>), dim3(grid), dim3(256), 0, stream, t, d, c);
             const int rc = fstx_internal::check_launch("newton_schulz_kernel");
             if (rc < 0 || sum_tiles == 0) return rc;
         }
@@ -1053,31 +1018,28 @@ struct Launcher {
             wgs += (tiles_of<kPhase, TR, TC>(t.job[i].p, t.job[i].q) - d.whole[i]) * (TR / 32) * (TC / 32);
         }
         fstx_internal::Range range("fstx join_pieces_kernel: phase %u, %u workgroups", kPhase, wgs);
-        hipLaunchKernelGGL((join_pieces_kernel<kPhase, TR, TC, Terms>), dim3(wgs), dim3(64), 0, stream, t, d, c);
+        hipLaunchKernelGGL((join_pieces_kernel<kPhase, TR, TC>), dim3(wgs), dim3(64), 0, stream, t, d, c);
         return fstx_internal::check_launch("join_pieces_kernel");
     }
 
-    template <uint32_t kPhase, uint32_t Terms> int phase(const Coefficients &c) {
-        const double t256 = deal<kPhase, 256, 256, Terms>(), t128 = deal<kPhase, 256, 128, Terms>(), t = deal<kPhase, 128, 128, Terms>(),
-                     small = deal<kPhase, 64, 64, Terms>();
-        if (small <= t && small <= t128 && small <= t256) return launch<kPhase, 64, 64, Terms>(c);
-        if (t <= t128 && t <= t256) return launch<kPhase, 128, 128, Terms>(c);
-        return t128 <= t256 ? launch<kPhase, 256, 128, Terms>(c) : launch<kPhase, 256, 256, Terms>(c);
+    template <uint32_t kPhase> int phase(const Coefficients &c) {
+        const double t256 = deal<kPhase, 256, 256>(), t128 = deal<kPhase, 256, 128>(), t = deal<kPhase, 128, 128>(), small = deal<kPhase, 64, 64>();
+        if (small <= t && small <= t128 && small <= t256) return launch<kPhase, 64, 64>(c);
+        if (t <= t128 && t <= t256) return launch<kPhase, 128, 128>(c);
+        return t128 <= t256 ? launch<kPhase, 256, 128>(c) : launch<kPhase, 256, 256>(c);
     }
-    template <uint32_t kPhase> int phase(bool one, const Coefficients &c) { return one ? phase<kPhase, 1>(c) : phase<kPhase, 2>(c); }
 
-    int steps(const float *coefficients, uint32_t count, uint64_t one_term) {
+    int steps(const float *coefficients, uint32_t count) {
         for (uint32_t step = 0; step < count; ++step) {
             const float a = coefficients[3 * step], b = coefficients[3 * step + 1], c = coefficients[3 * step + 2];
             // B is held times this: its entries stay below fp16's largest while singular values are below sqrt(2)
             const float scale_b = power_of_two_below(30000.0 / (2.0 * fabs((double)b) + 4.0 * fabs((double)c) + 0.01));
-            const bool last = step + 1 == count, one = one_term >> step & 1;
-            const uint32_t current = step & 1, next_both = !last && !(one_term >> (step + 1) & 1);
+            const uint32_t current = step & 1;
             int rc;
-            if ((rc = phase<kGram>(one, Coefficients{0, kScaleA, current, 0, 0})) < 0) return rc;
-            if ((rc = phase<kPoly>(one, Coefficients{b * scale_b / kScaleA, c * scale_b / (kScaleA * kScaleA), current, !one, 0})) < 0) return rc;
-            const Coefficients apply{a, 1.0f / scale_b, current, !last || !one, next_both};
-            if ((rc = last ? phase<kLast>(one, apply) : phase<kApply>(one, apply)) < 0) return rc;
+            if ((rc = phase<kGram>(Coefficients{0, kScaleA, current})) < 0) return rc;
+            if ((rc = phase<kPoly>(Coefficients{b * scale_b / kScaleA, c * scale_b / (kScaleA * kScaleA), current})) < 0) return rc;
+            const Coefficients apply{a, 1.0f / scale_b, current};
+            if ((rc = step + 1 == count ? phase<kLast>(apply) : phase<kApply>(apply)) < 0) return rc;
         }
         return 0;
     }
@@ -1111,17 +1073,13 @@ struct Launcher {
     }
 };
 
-// The matrices of one set of launches: those from `first` on that take one term in the same steps as `first` (so
-// that what a matrix is rounded to does not depend on what else is in the call), as many as fit.
-// Returns where the next set of that kind begins.
-uint32_t next_set(const fstx_orthogonalize_desc *descs, uint32_t n, const float *coefficients, uint32_t steps, uint32_t first, char *at, Launcher *set,
-                  uint64_t *bytes) {
-    const uint64_t kind = one_term_steps(descs[first], coefficients, steps);
+// The matrices of one set of launches: as many from `first` on as fit.  Returns where the next set begins.
+uint32_t next_set(const fstx_orthogonalize_desc *descs, uint32_t n, uint32_t first, char *at, Launcher *set, uint64_t *bytes) {
     *bytes = 0;
     set->n = 0;
     for (uint32_t k = 0; k < kMaxJobs; ++k) set->t.first[k] = 0xffffffffu;
     for (uint32_t i = first; i < n; ++i) {
-        if (empty(descs[i]) || slim(descs[i]) || one_term_steps(descs[i], coefficients, steps) != kind) continue;
+        if (empty(descs[i]) || slim(descs[i])) continue;
         const uint64_t need = Sides(descs[i]).bytes();
         if (set->n == kMaxJobs || (set->n && *bytes + need > kChunkBytes)) return i;
         set->add(descs[i], at + *bytes);
@@ -1129,28 +1087,6 @@ uint32_t next_set(const fstx_orthogonalize_desc *descs, uint32_t n, const float 
     }
     return n;
 }
-
-// The first descriptor from `from` on that begins the sets of another kind (`n`: there is none).  Kinds met so far are
-// kept; behind the last one that there is room for, the earlier descriptors are looked through.
-struct Kinds {
-    uint64_t met[32];
-    uint32_t n = 0;
-    uint32_t next(const fstx_orthogonalize_desc *descs, uint32_t count, const float *coefficients, uint32_t steps, uint32_t from) {
-        for (uint32_t i = from; i < count; ++i) {
-            if (empty(descs[i]) || slim(descs[i])) continue;
-            const uint64_t kind = one_term_steps(descs[i], coefficients, steps);
-            bool taken = false;
-            for (uint32_t k = 0; k < n; ++k) taken = taken || met[k] == kind;
-            if (!taken && n < 32) {
-                met[n++] = kind;
-                return i;
-            }
-            for (uint32_t j = 0; j < i && !taken; ++j) taken = !empty(descs[j]) && !slim(descs[j]) && one_term_steps(descs[j], coefficients, steps) == kind;
-            if (!taken) return i;
-        }
-        return count;
-    }
-};
 
 // Slim matrices from `first` on, as many as one set of launches takes; returns where the next set begins.
 uint32_t slim_set(const fstx_orthogonalize_desc *descs, uint32_t n, uint32_t first, char *at, SlimJobs *t, uint64_t *bytes) {
@@ -1219,18 +1155,15 @@ extern "C" int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *d
         first = slim_set(descs, n, first, nullptr, nullptr, &bytes);
         if (bytes > most) most = bytes;
     }
-    Kinds kinds;
-    for (uint32_t i = 0; (i = kinds.next(descs, n, coefficients, steps, i)) < n; ++i) {
-        for (uint32_t first = i; first < n;) {
-            Launcher set;
-            set.d.dies_log2 = fstx_internal::dies_log2();
-            uint64_t bytes;
-            const uint64_t kind = one_term_steps(descs[first], coefficients, steps);
-            first = next_set(descs, n, coefficients, steps, first, nullptr, &set, &bytes);
-            const int planned = set.steps(coefficients, steps, kind);
-            if (planned < 0) return planned;
-            if (bytes + set.sum_bytes > most) most = bytes + set.sum_bytes;
-        }
+    for (uint32_t first = 0; first < n;) {
+        Launcher set;
+        set.d.dies_log2 = fstx_internal::dies_log2();
+        uint64_t bytes;
+        first = next_set(descs, n, first, nullptr, &set, &bytes);
+        if (set.n == 0) break;
+        const int planned = set.steps(coefficients, steps);
+        if (planned < 0) return planned;
+        if (bytes + set.sum_bytes > most) most = bytes + set.sum_bytes;
     }
     return (int64_t)most;
 }
@@ -1249,34 +1182,31 @@ extern "C" int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t
         const int rc = slim_launch(t, coefficients, steps, eps, static_cast<hipStream_t>(stream));
         if (rc < 0) return rc;
     }
-    Kinds kinds;
-    for (uint32_t i = 0; (i = kinds.next(descs, n, coefficients, steps, i)) < n; ++i) {
-        for (uint32_t first = i; first < n;) {
-            Launcher set;
-            set.d.dies_log2 = fstx_internal::dies_log2();
-            set.stream = static_cast<hipStream_t>(stream);
-            set.run = true;
-            uint64_t bytes;
-            const uint64_t kind = one_term_steps(descs[first], coefficients, steps);
-            first = next_set(descs, n, coefficients, steps, first, static_cast<char *>(workspace), &set, &bytes);
-            set.d.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + bytes);
-            uint64_t grid = 0;
-            for (uint32_t k = 0; k < set.n; ++k) {
-                set.t.first[k] = (uint32_t)grid;
-                grid += set.t.job[k].n_partials;
-            }
-            hipLaunchKernelGGL(sum_squares_kernel, dim3((uint32_t)grid), dim3(256), 0, set.stream, set.t);
-            int rc = fstx_internal::check_launch("sum_squares_kernel");
-            if (rc < 0) return rc;
-            grid = 0;
-            for (uint32_t k = 0; k < set.n; ++k) {
-                set.t.first[k] = (uint32_t)grid;
-                grid += (uint64_t)(pad_to(set.t.job[k].p, kPadP) / 32) * (pad_to(set.t.job[k].q, kPadQ) / 32) / 4;
-            }
-            hipLaunchKernelGGL(first_operands_kernel, dim3((uint32_t)grid), dim3(256), 0, set.stream, set.t, eps, (uint32_t)!(kind & 1));
-            if ((rc = fstx_internal::check_launch("first_operands_kernel")) < 0) return rc;
-            if ((rc = set.steps(coefficients, steps, kind)) < 0) return rc;
+    for (uint32_t first = 0; first < n;) {
+        Launcher set;
+        set.d.dies_log2 = fstx_internal::dies_log2();
+        set.stream = static_cast<hipStream_t>(stream);
+        set.run = true;
+        uint64_t bytes;
+        first = next_set(descs, n, first, static_cast<char *>(workspace), &set, &bytes);
+        if (set.n == 0) break;
+        set.d.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + bytes);
+        uint64_t grid = 0;
+        for (uint32_t k = 0; k < set.n; ++k) {
+            set.t.first[k] = (uint32_t)grid;
+            grid += set.t.job[k].n_partials;
         }
+        hipLaunchKernelGGL(sum_squares_kernel, dim3((uint32_t)grid), dim3(256), 0, set.stream, set.t);
+        int rc = fstx_internal::check_launch("sum_squares_kernel");
+        if (rc < 0) return rc;
+        grid = 0;
+        for (uint32_t k = 0; k < set.n; ++k) {
+            set.t.first[k] = (uint32_t)grid;
+            grid += (uint64_t)(pad_to(set.t.job[k].p, kPadP) / 32) * (pad_to(set.t.job[k].q, kPadQ) / 32) / 4;
+        }
+        hipLaunchKernelGGL(first_operands_kernel, dim3((uint32_t)grid), dim3(256), 0, set.stream, set.t, eps);
+        if ((rc = fstx_internal::check_launch("first_operands_kernel")) < 0) return rc;
+        if ((rc = set.steps(coefficients, steps)) < 0) return rc;
     }
     return 0;
 }

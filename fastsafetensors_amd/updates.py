@@ -243,9 +243,8 @@ def orthogonalize(
     Returns new tensors of the updates' shapes and types, or fills ``outs`` (contiguous rows or
     contiguous columns; an update may be its own ``out``, but not overlap it partly).  One tensor in, one tensor out; a sequence gives a list.
     The matrices of one call run together, so that small ones share launches.  All are checked before
-    anything runs.  The iterates are held in 22 bits and products are as accurate as 32-bit ones, except where
-    shorter operands (11 bits) cannot be told from that in a result of the update's type: in steps in which the
-    product is a small part of the sum, and in the last step of a bf16 update.
+    anything runs.  The iterates and the operands of all products are held in 22 bits, sums in 32, whatever the
+    update's type; the result is rounded to it once.
 
     Up to 32 rows or columns everything is done in 64 bits.  A call takes 12 bytes of workspace per element of its matrices and
     8 per element of their squares, up to 4 GiB and more only for a matrix that alone needs more.
