@@ -695,20 +695,28 @@ __global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Dea
 // Up to 32 rows the whole iteration fits one workgroup when it is done on the Gram matrix M = G G^T in 64 bits: X is Q G with
 // Q a polynomial of M, so that a step is P = a I + b A + c A^2, Q <- P Q, A <- P A P, which all commute.  Squaring the
 // singular values costs half of the digits, which 64 bits have to spare and two fp16 terms have not: of a [1, 1] fp32
-// update they got 1.6e-6 of the value wrong, and this 4e-8.  It is three launches whatever the number of steps, and reads the
-// update twice: with five steps a [1, 700] fp32 update takes 22 us instead of 101, [32, 4096] 31 instead of 119 and
+// update they got 1.6e-6 of the value wrong, and this 4e-8.
+//
+// P A P loses that A is X X^T, whose eigenvalues are never negative: what rounding leaves of an eigenvalue of zero, +-2^-53,
+// grows by a^2 a step like that of any small direction, but a negative one without end (rank 1 and twenty steps of a = 3.4445: 1e40).
+// So steps are taken in runs in which a direction grows by kSlimGrowth at most, 2^26 times 2^-53 of an eigenvalue; between two runs
+// X = Q X is made, in 64 bits, and A taken from it anew.  The nine steps of a polar factor are one run.
+//
+// A run is three launches and reads the update twice: with five steps a [1, 700] fp32 update takes 22 us instead of 101, [32, 4096] 31 instead of 119 and
 // [32, 28672] 50 instead of 287.  At 64 rows one workgroup's products would take as long as the launches they save.
 // The partial sums of M are added in a fixed order.
 
 constexpr uint32_t kSlim = 32;      // rows at most
 constexpr uint32_t kSlimJobs = 32;
 constexpr uint32_t kSlimParts = 128; // workgroups that share the columns of one matrix
+constexpr double kSlimGrowth = 8192.0;
 
 struct alignas(32) SlimJob {
     const char *src;
     char *dst;
     double *grams; // n_parts of kSlim x kSlim
     double *q;     // kSlim x kSlim
+    double *x;     // p x q_cols, what the runs before have made of X (more than one run only)
     uint64_t x_row, x_col, dst_pitch; // elements, elements, bytes
     uint32_t p, q_cols, type, flipped, n_parts, pad;
 };
@@ -729,24 +737,40 @@ __device__ __forceinline__ uint32_t slim_job_of(const SlimJobs &t, uint32_t b) {
 using f64x4 = __attribute__((__vector_size__(4 * sizeof(double)))) double;
 __device__ __forceinline__ f64x4 mfma64(double a, double b, f64x4 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
 
+// Elements of X: in the first run those of G, in the type they have, later 64-bit ones
+template <bool kFirst> struct SlimElem { typedef float type; };
+template <> struct SlimElem<false> { typedef double type; };
+template <bool kFirst, uint32_t N, typename Row, typename Col>
+__device__ __forceinline__ void load_slim(const SlimJob &job, typename SlimElem<kFirst>::type (&x)[N], Row row, Col col) {
+    auto there = [&](uint32_t k) { return row(k) < job.p && col(k) < job.q_cols; };
+    if constexpr (kFirst) {
+        load_elems<N>(job.src, job.type, x, [&](uint32_t k) { return row(k) * job.x_row + col(k) * job.x_col; }, there);
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) x[k] = *(const FSTX_GLOBAL double *)(job.x + (there(k) ? row(k) * job.q_cols + col(k) : 0));
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) x[k] = there(k) ? x[k] : 0.0;
+    }
+}
+
 // A workgroup's share of M, 64 columns at a time, the next ones on their way while these are multiplied; a wave takes 16 of
 // them and the tiles on and below the diagonal.
-__global__ __launch_bounds__(256) void slim_gram_kernel(const SlimJobs t) {
+template <bool kFirst> __global__ __launch_bounds__(256) void slim_gram_kernel(const SlimJobs t) {
+    typedef typename SlimElem<kFirst>::type elem;
     constexpr uint32_t kWide = 64, kLoads = kSlim * kWide / 256;
     __shared__ union {
-        float x[kSlim][kWide + 4];
+        elem x[kSlim][kWide + 4];
         double sums[4][256];
     } lds;
     const uint32_t ji = slim_job_of(t, blockIdx.x);
     const SlimJob &job = t.job[ji];
     const uint32_t me = blockIdx.x - t.first[ji], p = job.p, n = job.q_cols, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const bool across = job.x_row < job.x_col; // columns of X lie along memory
-    float next[kLoads];
+    const bool across = kFirst && job.x_row < job.x_col; // columns of X lie along memory
+    elem next[kLoads];
     auto row_of = [&](uint32_t k) { return across ? (threadIdx.x + 256 * k) % kSlim : (threadIdx.x + 256 * k) / kWide; };
     auto col_of = [&](uint32_t k) { return across ? (threadIdx.x + 256 * k) / kSlim : (threadIdx.x + 256 * k) % kWide; };
     auto load = [&](uint64_t c0) {
-        load_elems<kLoads>(job.src, job.type, next, [&](uint32_t k) { return row_of(k) * job.x_row + (c0 + col_of(k)) * job.x_col; },
-                           [&](uint32_t k) { return row_of(k) < p && c0 + col_of(k) < n; });
+        load_slim<kFirst>(job, next, [&](uint32_t k) { return (uint64_t)row_of(k); }, [&](uint32_t k) { return c0 + col_of(k); });
     };
     f64x4 acc[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
     const uint64_t stride = (uint64_t)job.n_parts * kWide;
@@ -781,9 +805,9 @@ __global__ __launch_bounds__(256) void slim_gram_kernel(const SlimJobs t) {
     }
 }
 
-struct Steps {
+struct Steps { // of one run
     float c[3 * 64];
-    uint32_t n;
+    uint32_t n, first;
     float eps;
 };
 
@@ -803,7 +827,7 @@ __global__ __launch_bounds__(512) void slim_steps_kernel(const SlimJobs t, const
     __syncthreads();
     double trace = 0;
     for (uint32_t i = 0; i < p; ++i) trace += a[i][i];
-    const double factor = 1.0 / (sqrt(trace) + (double)steps.eps);
+    const double factor = steps.first ? 1.0 / (sqrt(trace) + (double)steps.eps) : 1.0;
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < kSlim * kSlim; e += 512) {
         a[e / kSlim][e % kSlim] *= factor * factor;
@@ -846,15 +870,14 @@ __global__ __launch_bounds__(512) void slim_steps_kernel(const SlimJobs t, const
     for (uint32_t e = threadIdx.x; e < kSlim * kSlim; e += 512) job.q[e] = q[e / kSlim][e % kSlim];
 }
 
-// The result, Q G: 16 columns by wave, read whole before they are written
-__global__ __launch_bounds__(256) void slim_apply_kernel(const SlimJobs t) {
+// Q X, into the result or, between two runs, into X: 16 columns by wave, read whole before they are written
+template <bool kFirst, bool kEnd> __global__ __launch_bounds__(256) void slim_apply_kernel(const SlimJobs t) {
     const uint32_t ji = slim_job_of(t, blockIdx.x);
     const SlimJob &job = t.job[ji];
     const uint32_t p = job.p, lane = threadIdx.x % 64, from = lane / 16;
     const uint64_t c = (uint64_t)(blockIdx.x - t.first[ji]) * 64 + threadIdx.x / 64 * 16 + lane % 16;
-    float g[kSlim / 4];
-    load_elems<kSlim / 4>(job.src, job.type, g, [&](uint32_t k) { return (4 * k + from) * job.x_row + c * job.x_col; },
-                          [&](uint32_t k) { return 4 * k + from < p && c < job.q_cols; });
+    typename SlimElem<kFirst>::type g[kSlim / 4];
+    load_slim<kFirst>(job, g, [&](uint32_t k) { return (uint64_t)(4 * k + from); }, [&](uint32_t) { return c; });
 #pragma unroll
     for (uint32_t i0 = 0; i0 < kSlim; i0 += 16) {
         if (i0 >= p) break;
@@ -865,6 +888,10 @@ __global__ __launch_bounds__(256) void slim_apply_kernel(const SlimJobs t) {
         for (uint32_t r = 0; r < 4; ++r) {
             const uint64_t i = i0 + 4 * r + from;
             if (i >= p || c >= job.q_cols) continue;
+            if constexpr (!kEnd) {
+                *(FSTX_GLOBAL double *)(job.x + i * job.q_cols + c) = d[r];
+                continue;
+            }
             char *at = job.dst + (job.flipped ? c : i) * job.dst_pitch;
             const uint64_t along = job.flipped ? i : c;
             if (job.type == FSTX_F32) ((FSTX_GLOBAL float *)at)[along] = (float)d[r];
@@ -1088,8 +1115,17 @@ uint32_t next_set(const fstx_orthogonalize_desc *descs, uint32_t n, uint32_t fir
     return n;
 }
 
+// Where the run of steps that begins with `first` ends
+uint32_t slim_run(const float *coefficients, uint32_t count, uint32_t first) {
+    double growth = 1.0;
+    uint32_t k = first;
+    do growth *= fmax(1.0, fabs((double)coefficients[3 * k]));
+    while (++k < count && growth * fmax(1.0, fabs((double)coefficients[3 * k])) <= kSlimGrowth);
+    return k;
+}
+
 // Slim matrices from `first` on, as many as one set of launches takes; returns where the next set begins.
-uint32_t slim_set(const fstx_orthogonalize_desc *descs, uint32_t n, uint32_t first, char *at, SlimJobs *t, uint64_t *bytes) {
+uint32_t slim_set(const fstx_orthogonalize_desc *descs, uint32_t n, bool one_run, uint32_t first, char *at, SlimJobs *t, uint64_t *bytes) {
     uint32_t k = 0;
     *bytes = 0;
     if (t)
@@ -1104,30 +1140,28 @@ uint32_t slim_set(const fstx_orthogonalize_desc *descs, uint32_t n, uint32_t fir
         const bool flipped = d.rows > d.cols;
         const uint64_t p = flipped ? d.cols : d.rows, q = flipped ? d.rows : d.cols, parts = (q + 255) / 256;
         const uint32_t n_parts = (uint32_t)(parts < kSlimParts ? parts : kSlimParts);
+        const uint64_t squares = (uint64_t)(n_parts + 1) * kSlim * kSlim, need = (squares + (one_run ? 0 : (p * q + 31) / 32 * 32)) * sizeof(double);
+        if (k && *bytes + need > kChunkBytes) return i;
         if (t) {
             double *space = reinterpret_cast<double *>(at + *bytes);
-            t->job[k] = SlimJob{static_cast<const char *>(d.src), static_cast<char *>(d.dst), space + kSlim * kSlim, space,
+            t->job[k] = SlimJob{static_cast<const char *>(d.src), static_cast<char *>(d.dst), space + kSlim * kSlim, space, space + squares,
                                 flipped ? d.src_col_stride : d.src_row_stride, flipped ? d.src_row_stride : d.src_col_stride,
                                 d.dst_pitch * size_of(d.type), (uint32_t)p, (uint32_t)q, d.type, flipped, n_parts, 0};
         }
-        *bytes += (uint64_t)(n_parts + 1) * kSlim * kSlim * sizeof(double);
+        *bytes += need;
         ++k;
     }
     return n;
 }
 
-int slim_launch(SlimJobs &t, const float *coefficients, uint32_t count, float eps, hipStream_t stream) {
-    Steps steps = {};
-    for (uint32_t i = 0; i < 3 * count; ++i) steps.c[i] = coefficients[i];
-    steps.n = count;
-    steps.eps = eps;
+template <bool kFirst> int slim_launch(SlimJobs &t, const Steps &steps, bool end, hipStream_t stream) {
     uint32_t n = 0, grid = 0;
     for (; n < kSlimJobs && t.job[n].p; ++n) {
         t.first[n] = grid;
         grid += t.job[n].n_parts;
     }
-    fstx_internal::Range range("fstx slim kernels: %u matrices", n);
-    hipLaunchKernelGGL(slim_gram_kernel, dim3(grid), dim3(256), 0, stream, t);
+    fstx_internal::Range range("fstx slim kernels: %u matrices, %u steps", n, steps.n);
+    hipLaunchKernelGGL((slim_gram_kernel<kFirst>), dim3(grid), dim3(256), 0, stream, t);
     int rc = fstx_internal::check_launch("slim_gram_kernel");
     if (rc < 0) return rc;
     hipLaunchKernelGGL(slim_steps_kernel, dim3(n), dim3(512), 0, stream, t, steps);
@@ -1137,8 +1171,23 @@ int slim_launch(SlimJobs &t, const float *coefficients, uint32_t count, float ep
         t.first[i] = grid;
         grid += (t.job[i].q_cols + 63) / 64;
     }
-    hipLaunchKernelGGL(slim_apply_kernel, dim3(grid), dim3(256), 0, stream, t);
+    if (end) hipLaunchKernelGGL((slim_apply_kernel<kFirst, true>), dim3(grid), dim3(256), 0, stream, t);
+    else hipLaunchKernelGGL((slim_apply_kernel<kFirst, false>), dim3(grid), dim3(256), 0, stream, t);
     return fstx_internal::check_launch("slim_apply_kernel");
+}
+
+int slim_runs(SlimJobs &t, const float *coefficients, uint32_t count, float eps, hipStream_t stream) {
+    for (uint32_t from = 0, to; from < count; from = to) {
+        to = slim_run(coefficients, count, from);
+        Steps steps = {};
+        for (uint32_t i = 0; i < 3 * (to - from); ++i) steps.c[i] = coefficients[3 * from + i];
+        steps.n = to - from;
+        steps.first = from == 0;
+        steps.eps = eps;
+        const int rc = from == 0 ? slim_launch<true>(t, steps, to == count, stream) : slim_launch<false>(t, steps, to == count, stream);
+        if (rc < 0) return rc;
+    }
+    return 0;
 }
 
 } // namespace
@@ -1149,10 +1198,11 @@ extern "C" int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *d
     if (steps < 1 || steps > kMaxSteps || !coefficients) return -FSTX_E_INVAL;
     for (uint32_t k = 0; k < 3 * steps; ++k)
         if (!isfinite(coefficients[k])) return -FSTX_E_INVAL;
+    const bool one_run = slim_run(coefficients, steps, 0) == steps;
     uint64_t most = 0;
     for (uint32_t first = 0; first < n;) {
         uint64_t bytes;
-        first = slim_set(descs, n, first, nullptr, nullptr, &bytes);
+        first = slim_set(descs, n, one_run, first, nullptr, nullptr, &bytes);
         if (bytes > most) most = bytes;
     }
     for (uint32_t first = 0; first < n;) {
@@ -1174,12 +1224,13 @@ extern "C" int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t
     if (need < 0) return (int)need;
     if (!(eps >= 0) || !isfinite(eps)) return -FSTX_E_INVAL;
     if (need && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (uint64_t)need)) return -FSTX_E_INVAL;
+    const bool one_run = slim_run(coefficients, steps, 0) == steps;
     for (uint32_t first = 0; first < n;) {
         SlimJobs t;
         uint64_t bytes;
-        first = slim_set(descs, n, first, static_cast<char *>(workspace), &t, &bytes);
+        first = slim_set(descs, n, one_run, first, static_cast<char *>(workspace), &t, &bytes);
         if (bytes == 0) continue;
-        const int rc = slim_launch(t, coefficients, steps, eps, static_cast<hipStream_t>(stream));
+        const int rc = slim_runs(t, coefficients, steps, eps, static_cast<hipStream_t>(stream));
         if (rc < 0) return rc;
     }
     for (uint32_t first = 0; first < n;) {

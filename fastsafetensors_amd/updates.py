@@ -246,7 +246,7 @@ def orthogonalize(
     anything runs.  The iterates and the operands of all products are held in 22 bits, sums in 32, whatever the
     update's type; the result is rounded to it once.
 
-    Up to 32 rows or columns everything is done in 64 bits.  A call takes 12 bytes of workspace per element of its matrices and
+    Up to 32 rows or columns everything is done in 64 bits.  Coefficients and eps are taken as 32-bit numbers.  A call takes 12 bytes of workspace per element of its matrices and
     8 per element of their squares, up to 4 GiB and more only for a matrix that alone needs more.
 
     The default coefficients leave singular values between 0.7 and 1.2, which is what an optimiser needs;
