@@ -1059,8 +1059,8 @@ struct Launcher {
     int steps(const float *coefficients, uint32_t count) {
         for (uint32_t step = 0; step < count; ++step) {
             const float a = coefficients[3 * step], b = coefficients[3 * step + 1], c = coefficients[3 * step + 2];
-            // B is held times this: its entries stay below fp16's largest while singular values are below sqrt(2)
-            const float scale_b = power_of_two_below(30000.0 / (2.0 * fabs((double)b) + 4.0 * fabs((double)c) + 0.01));
+            // B is held times this: its entries, |b| s^2 + |c| s^4 at most, stay below fp16's largest for singular values s of up to 2
+            const float scale_b = power_of_two_below(60000.0 / (4.0 * fabs((double)b) + 16.0 * fabs((double)c) + 0.01));
             const uint32_t current = step & 1;
             int rc;
             if ((rc = phase<kGram>(Coefficients{0, kScaleA, current})) < 0) return rc;

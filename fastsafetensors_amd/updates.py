@@ -251,7 +251,7 @@ def orthogonalize(
 
     The default coefficients leave singular values between 0.7 and 1.2, which is what an optimiser needs;
     ``POLAR_COEFFICIENTS`` drives them to 1.  Coefficients must keep the
-    iterates' singular values below about 2.  There is no gradient: tensors that require one are refused while
+    iterates' singular values at 2 or less.  There is no gradient: tensors that require one are refused while
     gradients are being recorded."""
     single = isinstance(updates, torch.Tensor)
     mats: List[torch.Tensor] = [updates] if single else list(updates)
