@@ -25,7 +25,8 @@
 // instead of 367.)
 // fp16 rather than bf16 terms because the iterates are bounded: entries of X are at most about
 // 1.2, they are held times a power of two near sqrt(p q) so that their typical size stays in the
-// middle of fp16's range; A and B are held times fixed powers of two likewise.
+// middle of fp16's range; A and B are held times powers of two likewise.  Where |G| is far below eps, or a step makes all singular values
+// small, these powers follow a bound of the singular values from step to step, for each matrix by itself: see Plan.
 //
 // Operand layout.  A matrix [R, K] that enters a product as rows x K is stored as blocks of 32
 // rows x 16 k in the lane order of v_mfma_f32_32x32x16 (lane: row lane % 32, k = 8 (lane / 32) + 0..7), 1 KiB
@@ -72,7 +73,7 @@ struct alignas(64) Job {
     half_t *x;        // [p, q]
     half_t *xt0, *xt1; // [q, p], the current one and the next in turn
     half_t *a, *b;    // [p, p]
-    double *partials;
+    double *partials; // later the matrix's Plan
     uint64_t x_row, x_col;   // strides of G seen as X, elements
     uint64_t dst_pitch;      // bytes
     uint32_t p, q;
@@ -82,6 +83,25 @@ struct alignas(64) Job {
     uint64_t pad[2];
 };
 static_assert(sizeof(Job) == 128, "20 of them fit the kernel arguments");
+
+struct Steps { // coefficients of a call, or of a run of steps
+    float c[3 * 64];
+    uint32_t n, first;
+    float eps;
+};
+
+// What one step multiplies with: B = own A + product A A, X = own X + product B X, as they are held
+struct StepPlan {
+    float poly_own, poly_product, apply_own, apply_product;
+};
+// Per matrix, over its partial sums of squares once these are added
+struct Plan {
+    float factor;
+    int32_t exponent; // X is G times factor 2^exponent
+    uint32_t pad[2];
+    StepPlan step[64];
+};
+static_assert(sizeof(Plan) <= kPartials * sizeof(double), "a plan takes the place of the partial sums");
 
 struct Jobs {
     Job job[kMaxJobs];
@@ -249,6 +269,48 @@ __global__ __launch_bounds__(256) void sum_squares_kernel(const Jobs t) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = sum;
     __syncthreads();
     if (threadIdx.x == 0) job.partials[me] = part[0] + part[1] + part[2] + part[3];
+}
+
+// The powers of two that a matrix's operands are held times, from a bound s of its singular values: |G| / (|G| + eps)
+// at first, |a| s + |b| s^3 + |c| s^5 behind a step.  X is held times scale 2^e, s 2^e being just below 1 (e = 0 from s = 1/2 on), A times
+// kScaleA 2^(2 e), and B times the power of two up to which 4 |b| + 16 |c|, its largest entry for s = 2, stays below fp16's
+// largest, and for e > 0 another 2^g that puts the bound |b| s^2 + |c| s^4 there.  Held times fixed powers of two instead, an
+// update of |G| = 10^-7 eps lost all but six digits of its bits in fp16's denormals, and one of 10^-8 eps was zero.
+// One wavefront per matrix; its partial sums are all read before the plan is written over them.
+__global__ __launch_bounds__(64) void plan_kernel(const Jobs t, const Steps steps) {
+    const Job job = fetch_job(t, blockIdx.x);
+    double sum = 0;
+    for (uint32_t i = threadIdx.x; i < job.n_partials; i += 64) sum += job.partials[i];
+    const double norm = sqrt(wave_sum(sum)), whole = norm + (double)steps.eps;
+    if (threadIdx.x) return;
+    auto exponent_of = [](double bound) { return bound > 0 && bound < 1 ? -ilogb(bound) - 1 : 0; };
+    FSTX_GLOBAL Plan *plan = (FSTX_GLOBAL Plan *)reinterpret_cast<Plan *>(job.partials);
+    double s = norm / whole; // (NaN, like what follows from it, where G holds infinities or NaN or |G| + eps is zero)
+    int e = exponent_of(s), shift = 0;
+    const double mantissa = frexp(whole, &shift); // 1 / (|G| + eps) may lie outside of what 32 bits hold, its mantissa and exponent do not
+    plan->factor = (float)((double)job.scale / mantissa);
+    plan->exponent = whole < HUGE_VAL ? e - shift : 0;
+    for (uint32_t k = 0; k < steps.n; ++k) {
+        const double a = steps.c[3 * k], b = steps.c[3 * k + 1], c = steps.c[3 * k + 2];
+        const bool linear = b == 0 && c == 0; // (B is zero)
+        const double top = linear ? 1.0 : 4.0 * fabs(b) + 16.0 * fabs(c);
+        const int held = ilogb(60000.0 / top);
+        int g = 0;
+        if (e > 0 && !linear) { // (exponents, because s^4 may be smaller than what 64 bits hold)
+            const double small = fmax(log2(fabs(b)) + 2.0 * log2(s), log2(fabs(c)) + 4.0 * log2(s));
+            g = (int)fmin(fmax(floor(log2(top) - 2.0 - small), 0.0), 4096.0);
+        }
+        const double next = s * (fabs(a) + s * s * (fabs(b) + s * s * fabs(c)));
+        const bool last = k + 1 == steps.n;
+        const int to = last ? -ilogb((double)job.scale) : exponent_of(next); // the result itself is not scaled
+        FSTX_GLOBAL StepPlan &p = plan->step[k];
+        p.poly_own = (float)ldexp(b / (double)kScaleA, held + g - 2 * e);
+        p.poly_product = (float)ldexp(c / ((double)kScaleA * (double)kScaleA), held + g - 4 * e);
+        p.apply_own = (float)ldexp(a, to - e);
+        p.apply_product = (float)ldexp(1.0, to - e - g - held);
+        s = next;
+        e = to;
+    }
 }
 
 // ------------------------------------------------------------ the products
@@ -451,7 +513,7 @@ __device__ __forceinline__ void exchange(const half_t (&in)[16], half_t (&out)[1
 }
 
 // X and X^T from G: a wavefront takes a 32 x 32 block, its lanes along the side along which memory runs.
-__global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const float eps) {
+__global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t) {
     const uint32_t ji = job_of(t, blockIdx.x);
     const Job job = fetch_job(t, ji);
     const uint32_t lane = threadIdx.x & 63;
@@ -466,14 +528,12 @@ __global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const
     float x[16];
     load_elems<16>(job.src, job.type, x, [&](uint32_t r) { return (uint64_t)row_of(r) * g.row_stride + (uint64_t)col * g.col_stride; },
                    [&](uint32_t r) { return row_of(r) < g.rows && col < g.cols; });
-    double sum = 0; // (while the elements are on their way)
-    for (uint32_t i = lane; i < job.n_partials; i += 64) sum += job.partials[i];
-    // 1 / (|G| + eps) may lie outside of what 32 bits hold, its mantissa and exponent do not
-    int exponent;
-    const float factor = (float)((double)job.scale / frexp(sqrt(wave_sum(sum)) + (double)eps, &exponent));
+    const FSTX_GLOBAL Plan *plan = (const FSTX_GLOBAL Plan *)reinterpret_cast<const Plan *>(job.partials);
+    const float factor = plan->factor;
+    const int exponent = plan->exponent;
     v16f v;
 #pragma unroll
-    for (uint32_t r = 0; r < 16; ++r) v[r] = __builtin_ldexpf(x[r], -exponent) * factor;
+    for (uint32_t r = 0; r < 16; ++r) v[r] = __builtin_ldexpf(x[r], exponent) * factor;
     half_t h[16], l[16], ht[16], lt[16];
     split(v, h, l);
     exchange(h, ht, lane);
@@ -490,10 +550,23 @@ __global__ __launch_bounds__(256) void first_operands_kernel(const Jobs t, const
 
 enum Phase : uint32_t { kGram, kPoly, kApply, kLast };
 
-struct Coefficients {
-    float own, product;  // result = own * (what is there) + product * (sum of the products)
-    uint32_t current;    // which of xt0, xt1 is the current one
+struct At {
+    uint32_t step;
+    __device__ uint32_t current() const { return step & 1; } // which of xt0, xt1 is the current one
 };
+
+// result = own * (what is there) + product * (sum of the products)
+struct Coefficients {
+    float own, product;
+};
+template <uint32_t kPhase> __device__ __forceinline__ Coefficients coefficients_of(const Job &job, const At &at) {
+    if constexpr (kPhase == kGram) {
+        return Coefficients{0.0f, kScaleA / (job.scale * job.scale)};
+    } else {
+        const FSTX_GLOBAL StepPlan &p = ((const FSTX_GLOBAL Plan *)reinterpret_cast<const Plan *>(job.partials))->step[at.step];
+        return kPhase == kPoly ? Coefficients{p.poly_own, p.poly_product} : Coefficients{p.apply_own, p.apply_product};
+    }
+}
 
 // Tiles of a symmetric matrix that reach on or below the diagonal, row by row: row i has kAspect (i + 1) of
 // them, a tile being kAspect times as high as wide.
@@ -519,13 +592,13 @@ __device__ __forceinline__ void store_rows(char *at, uint32_t col, uint64_t pitc
 
 // What is there already where block (rb, cb) of a product goes: A's block, or X's
 template <uint32_t kPhase>
-__device__ __forceinline__ RawBlock own_block(const Job &job, const Coefficients &c, uint32_t rb, uint32_t cb, uint32_t lane) {
+__device__ __forceinline__ RawBlock own_block(const Job &job, const At &step, uint32_t rb, uint32_t cb, uint32_t lane) {
     const uint32_t p_blocks = pad_to(job.p, kPadP) / 16, q_blocks = pad_to(job.q, kPadQ) / 16; // as stored
     if constexpr (kPhase == kGram) {
         return RawBlock{};
     } else if constexpr (kPhase == kLast) {
         const bool flipped = job.flipped;
-        return load_block(pick<const half_t *>(flipped, job.x, pick(c.current, job.xt1, job.xt0)), plane_of(p_blocks, q_blocks), pick(flipped, rb, cb), pick(flipped, cb, rb),
+        return load_block(pick<const half_t *>(flipped, job.x, pick(step.current(), job.xt1, job.xt0)), plane_of(p_blocks, q_blocks), pick(flipped, rb, cb), pick(flipped, cb, rb),
                           pick(flipped, q_blocks, p_blocks), lane);
     } else {
         return load_block(kPhase == kPoly ? job.a : job.x, plane_of(p_blocks, kPhase == kPoly ? p_blocks : q_blocks), rb, cb,
@@ -536,7 +609,7 @@ __device__ __forceinline__ RawBlock own_block(const Job &job, const Coefficients
 // What becomes of one 32 x 32 block of a product. `v` is laid out with lanes along rows (the transposed
 // product), in the last step of a matrix that is not flipped with lanes along columns.
 template <uint32_t kPhase>
-__device__ __forceinline__ void finish_block(const Job &job, const Coefficients &c, uint32_t rb, uint32_t cb, v16f v, const RawBlock &there, uint32_t lane) {
+__device__ __forceinline__ void finish_block(const Job &job, const At &step, const Coefficients &c, uint32_t rb, uint32_t cb, v16f v, const RawBlock &there, uint32_t lane) {
     const uint32_t p_blocks = pad_to(job.p, kPadP) / 16, q_blocks = pad_to(job.q, kPadQ) / 16;
     if constexpr (kPhase == kLast) {
         // lanes run along the contiguous side of the destination: 64 or 128 contiguous bytes per row
@@ -544,15 +617,14 @@ __device__ __forceinline__ void finish_block(const Job &job, const Coefficients 
         const uint32_t along = pick(flipped, rb, cb) * 32 + (lane & 31), first = pick(flipped, cb, rb) * 32 + 4 * (lane >> 5);
         const uint32_t rows = pick(flipped, job.q, job.p), cols = pick(flipped, job.p, job.q);
         if (along >= cols) return;
-        const float own = c.own / job.scale, product = c.product / job.scale; // (powers of two)
         const v16f x = value_of(there);
         char *at = job.dst + (uint64_t)first * job.dst_pitch;
-        if (job.type == FSTX_F32) store_rows<float>(at, along, job.dst_pitch, first, rows, x, v, own, product);
-        else if (job.type == FSTX_BF16) store_rows<__bf16>(at, along, job.dst_pitch, first, rows, x, v, own, product);
-        else store_rows<half_t>(at, along, job.dst_pitch, first, rows, x, v, own, product);
+        if (job.type == FSTX_F32) store_rows<float>(at, along, job.dst_pitch, first, rows, x, v, c.own, c.product);
+        else if (job.type == FSTX_BF16) store_rows<__bf16>(at, along, job.dst_pitch, first, rows, x, v, c.own, c.product);
+        else store_rows<half_t>(at, along, job.dst_pitch, first, rows, x, v, c.own, c.product);
     } else {
         if constexpr (kPhase == kGram) {
-            v *= c.product / (job.scale * job.scale);
+            v *= c.product;
         } else {
             const v16f own = value_of(there);
 #pragma unroll
@@ -566,7 +638,7 @@ __device__ __forceinline__ void finish_block(const Job &job, const Coefficients 
         if (kPhase == kApply || cb != rb) {
             exchange(h, ht, lane);
             exchange(l, lt, lane);
-            store_block(kPhase == kApply ? pick(c.current, job.xt0, job.xt1) : to, plane, cb, rb, p_blocks, lane, ht, lt);
+            store_block(kPhase == kApply ? pick(step.current(), job.xt0, job.xt1) : to, plane, cb, rb, p_blocks, lane, ht, lt);
         }
     }
 }
@@ -592,7 +664,7 @@ __device__ __forceinline__ void place_of(const Job &job, uint32_t tile, uint32_t
 }
 
 template <uint32_t kPhase, uint32_t TR, uint32_t TC>
-__global__ __launch_bounds__(256, (Product<TR, TC>::kWaves)) void newton_schulz_kernel(const Jobs t, const Deal deal, const Coefficients c) {
+__global__ __launch_bounds__(256, (Product<TR, TC>::kWaves)) void newton_schulz_kernel(const Jobs t, const Deal deal, const At step) {
     typedef Product<TR, TC> Prod;
     constexpr uint32_t kNR = Prod::kNR, kNC = Prod::kNC;
     __shared__ __attribute__((aligned(1024))) half_t lds[Prod::kBufs * Prod::kStage];
@@ -619,7 +691,7 @@ __global__ __launch_bounds__(256, (Product<TR, TC>::kWaves)) void newton_schulz_
     const uint32_t from = partial ? (uint32_t)((uint64_t)stages * part / deal.split) : 0;
     const uint32_t to = partial ? (uint32_t)((uint64_t)stages * (part + 1) / deal.split) : stages;
     const half_t *left = kPhase == kGram ? job.x : kPhase == kPoly ? job.a : job.b;
-    const half_t *right = kPhase == kGram ? job.x : kPhase == kPoly ? job.a : pick(c.current, job.xt1, job.xt0);
+    const half_t *right = kPhase == kGram ? job.x : kPhase == kPoly ? job.a : pick(step.current(), job.xt1, job.xt0);
     const uint64_t row = (uint64_t)stored * kBlk, k0 = (uint64_t)from * Prod::kKb * kBlk;
     const uint32_t p_blocks = pad_to(job.p, kPadP) / 16, q_blocks = pad_to(job.q, kPadQ) / 16;
     const uint64_t left_plane = plane_of(p_blocks, kPhase == kGram ? q_blocks : p_blocks);
@@ -649,22 +721,23 @@ __global__ __launch_bounds__(256, (Product<TR, TC>::kWaves)) void newton_schulz_
     auto fetch_row = [&](uint32_t i) {
 #pragma unroll
         for (uint32_t j = 0; j < kNC; ++j)
-            if (!symmetric<kPhase>() || cb0 + j <= rb0 + i) there[i % 2][j] = own_block<kPhase>(job, c, rb0 + i, cb0 + j, lane);
+            if (!symmetric<kPhase>() || cb0 + j <= rb0 + i) there[i % 2][j] = own_block<kPhase>(job, step, rb0 + i, cb0 + j, lane);
     };
     fetch_row(0);
+    const Coefficients c = coefficients_of<kPhase>(job, step);
 #pragma unroll
     for (uint32_t i = 0; i < kNR; ++i) {
         if (i + 1 < kNR) fetch_row(i + 1);
 #pragma unroll
         for (uint32_t j = 0; j < kNC; ++j)
             if (!symmetric<kPhase>() || cb0 + j <= rb0 + i) // above the diagonal: written as the mirror of (cb, rb)
-                finish_block<kPhase>(job, c, rb0 + i, cb0 + j, acc[i][j], there[i % 2][j], lane);
+                finish_block<kPhase>(job, step, c, rb0 + i, cb0 + j, acc[i][j], there[i % 2][j], lane);
     }
 }
 
 // The tiles whose sums came in pieces: a wavefront per 32 x 32 block adds them in order.
 template <uint32_t kPhase, uint32_t TR, uint32_t TC>
-__global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Deal deal, const Coefficients c) {
+__global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Deal deal, const At step) {
     typedef Product<TR, TC> Prod;
     constexpr uint32_t kBlocks = TR / 32 * (TC / 32);
     const uint32_t ji = job_of(t, blockIdx.x);
@@ -677,7 +750,8 @@ __global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Dea
     const uint32_t wave = ri / Prod::kNR * 2 + ci / Prod::kNC, i = ri % Prod::kNR, j = ci % Prod::kNC;
     const float *at = deal.sums + ((uint64_t)deal.slot[ji] + (uint64_t)nth * deal.split) * (TR * TC) +
                       ((wave * Prod::kNR + i) * Prod::kNC + j) * 1024 + threadIdx.x * 4;
-    const RawBlock there = own_block<kPhase>(job, c, rb, cb, threadIdx.x);
+    const RawBlock there = own_block<kPhase>(job, step, rb, cb, threadIdx.x);
+    const Coefficients c = coefficients_of<kPhase>(job, step);
     v16f v = {};
 #pragma unroll 4
     for (uint32_t s = 0; s < deal.split; ++s, at += TR * TC)
@@ -687,7 +761,7 @@ __global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Dea
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) v[4 * g + e] += part[e];
         }
-    finish_block<kPhase>(job, c, rb, cb, v, there, threadIdx.x);
+    finish_block<kPhase>(job, step, c, rb, cb, v, there, threadIdx.x);
 }
 
 // ------------------------------------------------------------ slim matrices
@@ -804,12 +878,6 @@ template <bool kFirst> __global__ __launch_bounds__(256) void slim_gram_kernel(c
         if (tile == 1) out[j * kSlim + i] = sum;
     }
 }
-
-struct Steps { // of one run
-    float c[3 * 64];
-    uint32_t n, first;
-    float eps;
-};
 
 // One workgroup per matrix: Q.  Rows and columns from p on are zero throughout (those of P are not, but meet only zeros).
 __global__ __launch_bounds__(512) void slim_steps_kernel(const SlimJobs t, const Steps steps) {
@@ -1026,7 +1094,7 @@ struct Launcher {
         return best;
     }
 
-    template <uint32_t kPhase, uint32_t TR, uint32_t TC> int launch(const Coefficients &c) {
+    template <uint32_t kPhase, uint32_t TR, uint32_t TC> int launch(const At &step) {
         deal<kPhase, TR, TC>();
         if (!run) {
             const uint64_t bytes = sum_tiles * TR * TC * sizeof(float);
@@ -1035,7 +1103,7 @@ struct Launcher {
         }
         {
             fstx_internal::Range range("fstx newton_schulz_kernel: phase %u, %u matrices, %u workgroups, tiles of %u x %u", kPhase, n, grid, TR, TC);
-            hipLaunchKernelGGL((newton_schulz_kernel<kPhase, TR, TC>), dim3(grid), dim3(256), 0, stream, t, d, c);
+            hipLaunchKernelGGL((newton_schulz_kernel<kPhase, TR, TC>), dim3(grid), dim3(256), 0, stream, t, d, step);
             const int rc = fstx_internal::check_launch("newton_schulz_kernel");
             if (rc < 0 || sum_tiles == 0) return rc;
         }
@@ -1045,28 +1113,23 @@ struct Launcher {
             wgs += (tiles_of<kPhase, TR, TC>(t.job[i].p, t.job[i].q) - d.whole[i]) * (TR / 32) * (TC / 32);
         }
         fstx_internal::Range range("fstx join_pieces_kernel: phase %u, %u workgroups", kPhase, wgs);
-        hipLaunchKernelGGL((join_pieces_kernel<kPhase, TR, TC>), dim3(wgs), dim3(64), 0, stream, t, d, c);
+        hipLaunchKernelGGL((join_pieces_kernel<kPhase, TR, TC>), dim3(wgs), dim3(64), 0, stream, t, d, step);
         return fstx_internal::check_launch("join_pieces_kernel");
     }
 
-    template <uint32_t kPhase> int phase(const Coefficients &c) {
+    template <uint32_t kPhase> int phase(const At &step) {
         const double t256 = deal<kPhase, 256, 256>(), t128 = deal<kPhase, 256, 128>(), t = deal<kPhase, 128, 128>(), small = deal<kPhase, 64, 64>();
-        if (small <= t && small <= t128 && small <= t256) return launch<kPhase, 64, 64>(c);
-        if (t <= t128 && t <= t256) return launch<kPhase, 128, 128>(c);
-        return t128 <= t256 ? launch<kPhase, 256, 128>(c) : launch<kPhase, 256, 256>(c);
+        if (small <= t && small <= t128 && small <= t256) return launch<kPhase, 64, 64>(step);
+        if (t <= t128 && t <= t256) return launch<kPhase, 128, 128>(step);
+        return t128 <= t256 ? launch<kPhase, 256, 128>(step) : launch<kPhase, 256, 256>(step);
     }
 
-    int steps(const float *coefficients, uint32_t count) {
-        for (uint32_t step = 0; step < count; ++step) {
-            const float a = coefficients[3 * step], b = coefficients[3 * step + 1], c = coefficients[3 * step + 2];
-            // B is held times this: its entries, |b| s^2 + |c| s^4 at most, stay below fp16's largest for singular values s of up to 2
-            const float scale_b = power_of_two_below(60000.0 / (4.0 * fabs((double)b) + 16.0 * fabs((double)c) + 0.01));
-            const uint32_t current = step & 1;
+    int steps(uint32_t count) {
+        for (uint32_t k = 0; k < count; ++k) {
+            const At step{k};
             int rc;
-            if ((rc = phase<kGram>(Coefficients{0, kScaleA, current})) < 0) return rc;
-            if ((rc = phase<kPoly>(Coefficients{b * scale_b / kScaleA, c * scale_b / (kScaleA * kScaleA), current})) < 0) return rc;
-            const Coefficients apply{a, 1.0f / scale_b, current};
-            if ((rc = step + 1 == count ? phase<kLast>(apply) : phase<kApply>(apply)) < 0) return rc;
+            if ((rc = phase<kGram>(step)) < 0 || (rc = phase<kPoly>(step)) < 0) return rc;
+            if ((rc = k + 1 == count ? phase<kLast>(step) : phase<kApply>(step)) < 0) return rc;
         }
         return 0;
     }
@@ -1113,6 +1176,15 @@ uint32_t next_set(const fstx_orthogonalize_desc *descs, uint32_t n, uint32_t fir
         *bytes += need;
     }
     return n;
+}
+
+Steps steps_of(const float *coefficients, uint32_t n, bool first, float eps) {
+    Steps steps = {};
+    for (uint32_t i = 0; i < 3 * n; ++i) steps.c[i] = coefficients[i];
+    steps.n = n;
+    steps.first = first;
+    steps.eps = eps;
+    return steps;
 }
 
 // Where the run of steps that begins with `first` ends
@@ -1179,11 +1251,7 @@ template <bool kFirst> int slim_launch(SlimJobs &t, const Steps &steps, bool end
 int slim_runs(SlimJobs &t, const float *coefficients, uint32_t count, float eps, hipStream_t stream) {
     for (uint32_t from = 0, to; from < count; from = to) {
         to = slim_run(coefficients, count, from);
-        Steps steps = {};
-        for (uint32_t i = 0; i < 3 * (to - from); ++i) steps.c[i] = coefficients[3 * from + i];
-        steps.n = to - from;
-        steps.first = from == 0;
-        steps.eps = eps;
+        const Steps steps = steps_of(coefficients + 3 * from, to - from, from == 0, eps);
         const int rc = from == 0 ? slim_launch<true>(t, steps, to == count, stream) : slim_launch<false>(t, steps, to == count, stream);
         if (rc < 0) return rc;
     }
@@ -1211,7 +1279,7 @@ extern "C" int64_t fstx_orthogonalize_workspace(const fstx_orthogonalize_desc *d
         uint64_t bytes;
         first = next_set(descs, n, first, nullptr, &set, &bytes);
         if (set.n == 0) break;
-        const int planned = set.steps(coefficients, steps);
+        const int planned = set.steps(steps);
         if (planned < 0) return planned;
         if (bytes + set.sum_bytes > most) most = bytes + set.sum_bytes;
     }
@@ -1233,6 +1301,7 @@ extern "C" int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t
         const int rc = slim_runs(t, coefficients, steps, eps, static_cast<hipStream_t>(stream));
         if (rc < 0) return rc;
     }
+    const Steps all = steps_of(coefficients, steps, true, eps);
     for (uint32_t first = 0; first < n;) {
         Launcher set;
         set.d.dies_log2 = fstx_internal::dies_log2();
@@ -1250,14 +1319,16 @@ extern "C" int fstx_orthogonalize(const fstx_orthogonalize_desc *descs, uint32_t
         hipLaunchKernelGGL(sum_squares_kernel, dim3((uint32_t)grid), dim3(256), 0, set.stream, set.t);
         int rc = fstx_internal::check_launch("sum_squares_kernel");
         if (rc < 0) return rc;
+        hipLaunchKernelGGL(plan_kernel, dim3(set.n), dim3(64), 0, set.stream, set.t, all);
+        if ((rc = fstx_internal::check_launch("plan_kernel")) < 0) return rc;
         grid = 0;
         for (uint32_t k = 0; k < set.n; ++k) {
             set.t.first[k] = (uint32_t)grid;
             grid += (uint64_t)(pad_to(set.t.job[k].p, kPadP) / 32) * (pad_to(set.t.job[k].q, kPadQ) / 32) / 4;
         }
-        hipLaunchKernelGGL(first_operands_kernel, dim3((uint32_t)grid), dim3(256), 0, set.stream, set.t, eps);
+        hipLaunchKernelGGL(first_operands_kernel, dim3((uint32_t)grid), dim3(256), 0, set.stream, set.t);
         if ((rc = fstx_internal::check_launch("first_operands_kernel")) < 0) return rc;
-        if ((rc = set.steps(coefficients, steps)) < 0) return rc;
+        if ((rc = set.steps(steps)) < 0) return rc;
     }
     return 0;
 }

@@ -244,7 +244,7 @@ def orthogonalize(
     contiguous columns; an update may be its own ``out``, but not overlap it partly).  One tensor in, one tensor out; a sequence gives a list.
     The matrices of one call run together, so that small ones share launches.  All are checked before
     anything runs.  The iterates and the operands of all products are held in 22 bits, sums in 32, whatever the
-    update's type; the result is rounded to it once.
+    update's type; the result is rounded to it once.  Updates far smaller than ``eps`` keep these bits.
 
     Up to 32 rows or columns everything is done in 64 bits.  Coefficients and eps are taken as 32-bit numbers.  A call takes 12 bytes of workspace per element of its matrices and
     8 per element of their squares, up to 4 GiB and more only for a matrix that alone needs more.

@@ -56,7 +56,9 @@ int fstx_merge_low_rank(const fstx_low_rank_desc *descs, uint32_t n, void *works
 /* dst = the nearest orthogonal matrix of src, approximated by `steps` Newton-Schulz steps:
  *   X = src / (|src|_F + eps);   per step (a, b, c):  A = X X^T,  X <- a X + (b A + c A A) X
  * with the shorter side as rows (orthogonal rows if rows <= cols, else orthogonal columns).  Iterates and
- * operands are held in 22 bits whatever the type; sums are held in 32 bits, the norm's in 64.  While the steps run the
+ * operands are held in 22 bits whatever the type, scaled by a bound of the singular values (|src| / (|src| + eps),
+ * then |a| s + |b| s^3 + |c| s^5 per step; a step that leaves X far below that, as a = 0 does to many small
+ * singular values, costs the bits between the two); sums are held in 32 bits, the norm's in 64.  While the steps run the
  * iterates' singular values must not exceed 2 (those of X start at 1 or less).  With up to 32 rows
  * or columns everything is done in 64 bits.  Infinities and NaN spread through the result
  * as they do in the formula. */
