@@ -269,7 +269,9 @@ class FilesBufferOnDevice:
         (default: every one of two dimensions, both larger than 1) becomes ``W + scale * s * O``, ``O`` being
         the orthogonal matrix nearest to ``D`` and ``s`` the mean of ``D``'s singular values: every direction that some
         checkpoint changed weighs the same, so that the strong directions of one task do not drown
-        the others.  The remaining tensors get the mean difference, ``W + scale * D / len(others)``.
+        the others (directions whose singular value is below 0.0005 of ``D``'s Frobenius norm count as
+        noise and weigh less).  Tensors whose rows are no map's directions, such as embeddings, are left out by
+        naming the others in ``orthogonal``.  The remaining tensors get the mean difference, ``W + scale * D / len(others)``.
 
         fp32, fp16 and bf16 tensors of the same type and shape everywhere; everything is checked before the
         first one changes, all work is queued on the current stream."""

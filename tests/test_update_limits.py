@@ -2,6 +2,8 @@
 """Workspaces and limits of the kernels that change weights; nothing is launched and no GPU is needed."""
 import ctypes
 
+import torch
+
 from fastsafetensors_amd import _native
 
 F32, F16, BF16 = (_native.ELEM_TYPES[k] for k in ("F32", "F16", "BF16"))
@@ -28,3 +30,23 @@ def test_slim_matrices_and_many_steps_take_room_for_the_iterate():
     one = need([polar] * 64, update(32, 1 << 20))
     assert one == 129 * 8192 + (32 << 23)
     assert need([polar] * 64, *[update(32, 1 << 20, i) for i in range(40)]) == (4 << 30) // one * one
+
+
+def test_coefficients_reach_what_is_said_of_them():
+    """Singular values relative to the Frobenius norm, on a grid of 2 * 10^6 over six decades (steps of 7e-6 of a value,
+    which slopes of up to 6000 turn into 4e-2 of it where a value is small, and into nothing that matters where it has converged)."""
+    from fastsafetensors_amd.updates import DEFAULT_COEFFICIENTS, POLAR_COEFFICIENTS
+
+    s = torch.logspace(-6, 0, 2_000_001, dtype=torch.float64)
+
+    def outcome(coefficients):
+        x = s
+        for a, b, c in coefficients:
+            x = a * x + b * x**3 + c * x**5
+            assert x.max() < 1.21  # and iterates stay below 2
+        return x
+
+    five, polar = outcome(DEFAULT_COEFFICIENTS), outcome(POLAR_COEFFICIENTS)
+    assert five[s >= 1.5e-3].min() >= 0.679 and abs(five[s <= 1e-3].max().item() - 0.47) < 0.01
+    assert ((polar - 1).abs()[s >= 5e-4] < 3e-4).all() and ((polar - 1).abs()[s >= 7e-4] < 1e-6).all()
+    assert abs(five[0].item() / 1e-6 - 484.9) < 0.5 and abs(polar[0].item() / 1e-6 - 5993) < 5  # a^5, times 1.875^4; cubic terms are below 1e-4 of it
