@@ -11,7 +11,7 @@ import contextlib
 import math
 import struct
 from dataclasses import dataclass
-from typing import Any, List, Optional, Sequence, Union
+from typing import Any, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -167,17 +167,24 @@ def _pack_plain(buf: bytearray, at: int, u: LowRankUpdate, device: torch.device,
         return False
 
 
-def _launch_low_rank(descs: Any, first: int, n: int, device: torch.device, need: int, stream: int) -> None:
+def _low_rank_calls(descs: Any, first: int, n: int, need: int) -> List[Tuple[Any, int, int]]:
+    """The library calls that ``descs`` are cut into: where they begin, how many, their workspace."""
     at = descs if first == 0 else _native.ctypes.cast(
         _native.ctypes.byref(descs, first * _DESC.size), _native.ctypes.POINTER(_native.FstxLowRankDesc))
     if need < 0:
         need = _native.merge_low_rank_workspace(at, n)
     if need > _WORKSPACE_BYTES and n > 1:
-        _launch_low_rank(descs, first, n // 2, device, -1, stream)
-        _launch_low_rank(descs, first + n // 2, n - n // 2, device, -1, stream)
-        return
-    space = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _native.merge_low_rank(at, n, 0 if space is None else space.data_ptr(), need, stream)
+        return _low_rank_calls(descs, first, n // 2, -1) + _low_rank_calls(descs, first + n // 2, n - n // 2, -1)
+    return [(at, n, need)]
+
+
+def _launch_low_rank(descs: Any, n: int, device: torch.device, need: int, stream: int) -> None:
+    calls = _low_rank_calls(descs, 0, n, need)
+    # one workspace for all of them, which follow each other on the stream: if there is no memory for it, nothing has changed
+    most = max(c[2] for c in calls)
+    space = torch.empty(most, dtype=torch.uint8, device=device) if most else None
+    for at, count, bytes_ in calls:
+        _native.merge_low_rank(at, count, 0 if space is None else space.data_ptr(), bytes_, stream)
 
 
 def _on_device(device: torch.device) -> Any:
@@ -213,7 +220,7 @@ def merge_low_rank(updates: Sequence[LowRankUpdate]) -> List[torch.Tensor]:
         raise ValueError(f"merge_low_rank: results overlap what other updates read or write, or a size is out of range ({e})") from None
     outs = [u.weight if u.out is None else u.out for u in updates]
     with _on_device(device):
-        _launch_low_rank(descs, 0, n, device, need, torch.cuda.current_stream(device).cuda_stream)
+        _launch_low_rank(descs, n, device, need, torch.cuda.current_stream(device).cuda_stream)
     torch.autograd.graph.increment_version(outs)
     return outs
 
