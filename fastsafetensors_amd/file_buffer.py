@@ -273,8 +273,9 @@ class FilesBufferOnDevice:
         noise and weigh less).  Tensors whose rows are no map's directions, such as embeddings, are left out by
         naming the others in ``orthogonal``.  The remaining tensors get the mean difference, ``W + scale * D / len(others)``.
 
-        fp32, fp16 and bf16 tensors of the same type and shape everywhere; everything is checked before the
-        first one changes, all work is queued on the current stream."""
+        fp32, fp16 and bf16 tensors of the same type and shape everywhere; everything is checked, and all memory
+        asked for, before the first one changes (8 bytes per element of the largest tensor, 12 more for a matrix and 8 per
+        element of its square, or what that comes to for matrices of 2^28 elements together); all work is queued on the current stream."""
         if not others:
             raise ValueError("merge_checkpoints: no checkpoints to merge")
         names = list(others[0].key_to_rank_lidx)

@@ -27,7 +27,7 @@ import torch
 from .. import _native
 from ..common import SingleGroup, TensorFrame
 from ..st_types import Device, DeviceType, DType, dtype_size
-from ..updates import MAX_SHORT_SIDE, MAX_SIDE, POLAR_COEFFICIENTS, LowRankUpdate, merge_low_rank, orthogonalize
+from ..updates import MAX_SHORT_SIDE, MAX_SIDE, POLAR_COEFFICIENTS, LowRankUpdate, Orthogonalization, merge_low_rank
 from . import FrameworkOpBase, ProcessGroupBase, TensorBase
 
 dtype_convert: Dict[DType, torch.dtype] = {
@@ -546,27 +546,54 @@ class TorchOp(FrameworkOpBase):
                 raise ValueError(f"a tensor of shape {tuple(w.shape)} on {w.device} cannot be orthogonalised")
             work.append((w, ts, orthogonal))
 
-        def delta(w: torch.Tensor, ts: List[torch.Tensor]) -> torch.Tensor:
-            out = torch.zeros(w.shape, dtype=torch.float32, device=w.device)
-            for t in ts:
-                out += t.float() - w.float()
-            return out
+        # All memory is asked for before the first tensor changes: differences and a second buffer as large, both of
+        # as many matrices at a time as _MERGE_ELEMS holds, and the workspace of the largest call.
+        groups: List[List[Tuple[torch.Tensor, List[torch.Tensor], int]]] = []
+        most = elems = 0
+        for w, ts, orthogonal in work:
+            if not w.numel():
+                continue
+            if orthogonal:
+                if not groups or elems + w.numel() > _MERGE_ELEMS:
+                    groups.append([])
+                    elems = 0
+                groups[-1].append((w, ts, elems))
+                elems += (w.numel() + 127) // 128 * 128  # each begins on 512 bytes
+                most = max(most, elems)
+            else:
+                most = max(most, w.numel())
+        if not most:
+            return
+        device = work[0][0].device
+        if any(w.device != device for w, _, _ in work):
+            raise ValueError("the tensors are on different devices")
+        differences, second = (torch.empty(most, dtype=torch.float32, device=device) for _ in range(2))
+
+        def part(flat: torch.Tensor, w: torch.Tensor, at: int = 0) -> torch.Tensor:
+            return flat[at : at + w.numel()].view(w.shape)
+
+        def difference(w: torch.Tensor, ts: List[torch.Tensor], d: torch.Tensor, other: torch.Tensor) -> None:
+            d.copy_(ts[0]).sub_(w)
+            for t in ts[1:]:
+                d.add_(other.copy_(t).sub_(w))
 
         with torch.no_grad():
+            calls = [Orthogonalization([part(differences, w, at) for w, _, at in group], POLAR_COEFFICIENTS, 1e-7,
+                                       [part(second, w, at) for w, _, at in group]) for group in groups]
+            space = torch.empty(max((c.need for c in calls), default=0), dtype=torch.uint8, device=device)
             for w, ts, orthogonal in work:
                 if not orthogonal and w.numel():
-                    w.copy_(w.float() + delta(w, ts) * (scale / len(ts)))
-            matrices = [(w, ts) for w, ts, orthogonal in work if orthogonal and w.numel()]
-            while matrices:  # as many at a time as fit next to the checkpoints
-                group, elems = [], 0
-                while matrices and (not group or elems + matrices[0][0].numel() <= _MERGE_ELEMS):
-                    group.append(matrices.pop(0))
-                    elems += group[-1][0].numel()
-                deltas = [delta(w, ts) for w, ts in group]
-                for (w, _), d, o in zip(group, deltas, orthogonalize(deltas, coefficients=POLAR_COEFFICIENTS)):
+                    d = part(differences, w)
+                    difference(w, ts, d, part(second, w))
+                    w.copy_(d.mul_(scale / len(ts)).add_(w))
+            for group, call in zip(groups, calls):
+                for (w, ts, _), d, o in zip(group, call.mats, call.outs):
+                    difference(w, ts, d, o)
+                call.launch(space)
+                for (w, _, _), d, o in zip(group, call.mats, call.outs):
                     # sum of the singular values = <d, o>; their mean keeps the update's size
-                    mean = (d * o).sum() / min(w.shape)
-                    w.copy_(w.float() + o * (scale * mean))
+                    mean = d.mul_(o).sum() / min(w.shape)
+                    w.copy_(o.mul_(scale * mean).add_(w))
 
     # ---- misc ------------------------------------------------------------------
     def synchronize(self, device: Device) -> None:

@@ -263,55 +263,73 @@ def orthogonalize(
     iterates' singular values at 2 or less.  There is no gradient: tensors that require one are refused while
     gradients are being recorded."""
     single = isinstance(updates, torch.Tensor)
-    mats: List[torch.Tensor] = [updates] if single else list(updates)
-    flat = [float(v) for step in coefficients for v in step]
-    if not all(len(step) == 3 for step in coefficients) or not 1 <= len(flat) // 3 <= 64:
-        raise ValueError("coefficients must be 1 to 64 triples (a, b, c)")
-    if not all(math.isfinite(v) for v in flat) or not (math.isfinite(eps) and eps >= 0):
-        raise ValueError("coefficients must be finite, eps finite and not negative")
-    if not all(abs(v) <= _LARGEST for v in (*flat, eps)):
-        raise ValueError("coefficients and eps must be 32-bit numbers")
     if outs is not None:
         outs = [outs] if single and isinstance(outs, torch.Tensor) else list(outs)
-        if len(outs) != len(mats):
-            raise ValueError(f"{len(outs)} outs for {len(mats)} updates")
-    if not mats:
-        return []
-    grad = torch.is_grad_enabled()
-    device: Optional[torch.device] = None
-    for i, g in enumerate(mats):
-        device = _on_gpu(g, "update", device, grad)
-        if g.dtype not in _FACTOR_TYPES:
-            raise TypeError(f"update is {g.dtype}; fp32, fp16 and bf16 are served")
-        if g.dim() != 2:
-            raise ValueError(f"update {tuple(g.shape)} does not have two dimensions")
+    call = Orthogonalization([updates] if single else list(updates), coefficients, eps, outs)
+    if call.device is not None:
+        call.launch(torch.empty(call.need, dtype=torch.uint8, device=call.device))
         if outs is not None:
-            _on_gpu(outs[i], "out", device, grad)
-            if outs[i].shape != g.shape or outs[i].dtype != g.dtype:
-                raise ValueError(f"out is {tuple(outs[i].shape)} {outs[i].dtype}, update {tuple(g.shape)} {g.dtype}")
-    given = outs is not None
-    if outs is None:
-        outs = [torch.empty(g.shape, dtype=g.dtype, device=device) for g in mats]
-    descs = (_native.FstxOrthogonalizeDesc * len(mats))()
-    for d, g, out in zip(descs, mats, outs):
-        if not _by_rows(out):  # the transposed problem is the same one
-            g, out = g.t(), out.t()
-            if not _by_rows(out):
-                raise ValueError("out must have contiguous rows or contiguous columns")
-        d.dst, d.src = out.data_ptr(), g.data_ptr()
-        d.rows, d.cols = g.shape
-        d.dst_pitch = _pitch(out, "out")
-        d.src_row_stride, d.src_col_stride = g.stride()
-        d.type = _FACTOR_TYPES[g.dtype]
-    triples, steps = (_native.ctypes.c_float * len(flat))(*flat), len(flat) // 3
-    with _on_device(device):
-        try:
-            need = _native.orthogonalize_workspace(descs, len(mats), triples, steps)
-        except _native.NativeError as e:
-            raise ValueError(f"orthogonalize: outs overlap each other or other updates, or a size is out of range ({e})") from None
-        space = torch.empty(need, dtype=torch.uint8, device=device)
-        _native.orthogonalize(descs, len(mats), triples, steps, float(eps), space.data_ptr() if need else 0, need,
-                              torch.cuda.current_stream(device).cuda_stream)
-    if given:
-        torch.autograd.graph.increment_version(outs)
-    return outs[0] if single else outs
+            torch.autograd.graph.increment_version(outs)
+    return call.outs[0] if single else call.outs
+
+
+class Orthogonalization:
+    """A checked call of ``orthogonalize``: ``need`` bytes of workspace, then ``launch``."""
+
+    def __init__(
+        self,
+        mats: List[torch.Tensor],
+        coefficients: Sequence[Sequence[float]],
+        eps: float,
+        outs: Optional[List[torch.Tensor]],
+    ) -> None:
+        flat = [float(v) for step in coefficients for v in step]
+        if not all(len(step) == 3 for step in coefficients) or not 1 <= len(flat) // 3 <= 64:
+            raise ValueError("coefficients must be 1 to 64 triples (a, b, c)")
+        if not all(math.isfinite(v) for v in flat) or not (math.isfinite(eps) and eps >= 0):
+            raise ValueError("coefficients must be finite, eps finite and not negative")
+        if not all(abs(v) <= _LARGEST for v in (*flat, eps)):
+            raise ValueError("coefficients and eps must be 32-bit numbers")
+        if outs is not None and len(outs) != len(mats):
+            raise ValueError(f"{len(outs)} outs for {len(mats)} updates")
+        grad = torch.is_grad_enabled()
+        device: Optional[torch.device] = None
+        for i, g in enumerate(mats):
+            device = _on_gpu(g, "update", device, grad)
+            if g.dtype not in _FACTOR_TYPES:
+                raise TypeError(f"update is {g.dtype}; fp32, fp16 and bf16 are served")
+            if g.dim() != 2:
+                raise ValueError(f"update {tuple(g.shape)} does not have two dimensions")
+            if outs is not None:
+                _on_gpu(outs[i], "out", device, grad)
+                if outs[i].shape != g.shape or outs[i].dtype != g.dtype:
+                    raise ValueError(f"out is {tuple(outs[i].shape)} {outs[i].dtype}, update {tuple(g.shape)} {g.dtype}")
+        if outs is None:
+            outs = [torch.empty(g.shape, dtype=g.dtype, device=device) for g in mats]
+        descs = (_native.FstxOrthogonalizeDesc * len(mats))()
+        for d, g, out in zip(descs, mats, outs):
+            if not _by_rows(out):  # the transposed problem is the same one
+                g, out = g.t(), out.t()
+                if not _by_rows(out):
+                    raise ValueError("out must have contiguous rows or contiguous columns")
+            d.dst, d.src = out.data_ptr(), g.data_ptr()
+            d.rows, d.cols = g.shape
+            d.dst_pitch = _pitch(out, "out")
+            d.src_row_stride, d.src_col_stride = g.stride()
+            d.type = _FACTOR_TYPES[g.dtype]
+        self.device, self.mats, self.outs, self.need = device, mats, outs, 0
+        self._args = (descs, len(mats), (_native.ctypes.c_float * len(flat))(*flat), len(flat) // 3)
+        self._eps = float(eps)
+        if device is None:
+            return
+        with _on_device(device):
+            try:
+                self.need = _native.orthogonalize_workspace(*self._args)
+            except _native.NativeError as e:
+                raise ValueError(f"orthogonalize: outs overlap each other or other updates, or a size is out of range ({e})") from None
+
+    def launch(self, space: torch.Tensor) -> None:
+        """Queue the work on the current stream, with the first ``need`` bytes of ``space``."""
+        with _on_device(self.device):
+            _native.orthogonalize(*self._args, self._eps, space.data_ptr() if self.need else 0, self.need,
+                                  torch.cuda.current_stream(self.device).cuda_stream)
