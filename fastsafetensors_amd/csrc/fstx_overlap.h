@@ -32,7 +32,10 @@ inline Block block_of(const void *p, uint64_t n0, uint64_t s0, uint64_t n1, uint
 
 inline bool overlap(const Block &a, const Block &b) {
     if (a.at >= b.end() || b.at >= a.end()) return false;
-    if (a.pitch != b.pitch || a.rows == 1 || b.rows == 1) return true; // spans that touch: not told apart further
+    // a single row has whatever pitch the other block has
+    if (a.rows == 1 && b.rows > 1 && a.pitch != b.pitch && a.width <= b.pitch) return overlap(Block{a.at, a.width, b.pitch, 1}, b);
+    if (b.rows == 1 && a.rows > 1 && a.pitch != b.pitch && b.width <= a.pitch) return overlap(a, Block{b.at, b.width, a.pitch, 1});
+    if (a.pitch != b.pitch) return true; // spans that touch: not told apart further
     if (b.at < a.at) return overlap(b, a);
     // rows of one tensor: b starts `shift` rows and `col` bytes behind a
     const uint64_t shift = (b.at - a.at) / a.pitch, col = (b.at - a.at) % a.pitch;

@@ -50,3 +50,31 @@ def test_coefficients_reach_what_is_said_of_them():
     assert five[s >= 1.5e-3].min() >= 0.679 and abs(five[s <= 1e-3].max().item() - 0.47) < 0.01
     assert ((polar - 1).abs()[s >= 5e-4] < 3e-4).all() and ((polar - 1).abs()[s >= 7e-4] < 1e-6).all()
     assert abs(five[0].item() / 1e-6 - 484.9) < 0.5 and abs(polar[0].item() / 1e-6 - 5993) < 5  # a^5, times 1.875^4; cubic terms are below 1e-4 of it
+
+
+def test_overlaps_are_those_of_the_bytes():
+    """Pairs of blocks, small enough to list their bytes: what overlaps is refused, and what does not is taken where both have
+    rows equally far apart or one is a single row (blocks of different pitches whose spans touch are not told apart)."""
+    import random
+
+    rng, base, fn = random.Random(5), 1 << 20, _native.lib().fstx_merge_low_rank_workspace
+    told = 0
+    for _ in range(20000):
+        blocks, descs = [], []
+        pitch = rng.randint(1, 9)
+        for i in range(2):
+            rows, own = rng.randint(1, 5), pitch if rng.random() < 0.7 else rng.randint(1, 9)
+            cols = rng.randint(1, own if rows > 1 else 9)
+            at = rng.randint(0, 40)
+            blocks.append((at, rows, cols, own))
+            descs.append(_native.FstxLowRankDesc(base + 2 * at, (2 + i) << 30, None, None, None, rows, cols, 0, own, cols, 0, 0, 0, 0, 1.0,
+                                                 BF16, BF16, BF16, 0, 0))
+        bytes_ = [{at + r * own + c for r in range(rows) for c in range(cols)} for at, rows, cols, own in blocks]
+        got = fn((_native.FstxLowRankDesc * 2)(*descs), 2)
+        (_, r0, c0, p0), (_, r1, c1, p1) = blocks
+        if bytes_[0] & bytes_[1]:
+            assert got == -10001, blocks
+        elif p0 == p1 or r0 == r1 == 1 or (r0 == 1 and c0 <= p1) or (r1 == 1 and c1 <= p0):
+            assert got == 0, blocks
+            told += 1
+    assert told > 5000
