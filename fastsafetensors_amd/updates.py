@@ -57,6 +57,8 @@ def _on_gpu(t: Any, what: str, device: Optional[torch.device], grad: bool) -> to
         raise ValueError(f"{what} is on {t.device}, the others are on {device}")
     if t.layout is not torch.strided:
         raise ValueError(f"{what} must be a dense tensor")
+    if t.is_neg():  # (the imaginary part of a conjugated tensor: its memory holds the other sign)
+        raise ValueError(f"{what} is a negated view: give its resolve_neg()")
     if grad and t.requires_grad:
         raise RuntimeError(f"{what} requires a gradient, which this call does not provide: use torch.no_grad()")
     return t.device
@@ -150,6 +152,7 @@ def _pack_plain(buf: bytearray, at: int, u: LowRankUpdate, device: torch.device,
             not -_LARGEST <= scale <= _LARGEST or m != m2 or n != n2 or r != r2 or one != 1 or out_one != 1 or src_pitch < n or dst_pitch < n
             or w.device != device or up.device != device or down.device != device
             or (grad and (w.requires_grad or up.requires_grad or down.requires_grad))
+            or w.is_neg() or up.is_neg() or down.is_neg() or out.is_neg() or (ws is not None and ws.is_neg())
         ):
             return False
         if wt == _E4M3:
