@@ -26,10 +26,12 @@
 //
 // Numerics.  MFMA products of bf16 / fp16 are exact in fp32 and are summed in fp32.  Factors of
 // f32 are split into bf16 terms x = h + m (+ l), each the rounding of what is left: bf16 because it
-// has f32's range.  Two terms (16 bits of each factor; h h + h m + m h, what is left out is below
-// 2^-16 of a product) for weights of 8 or 16 bits, whose own rounding is 2^-12 at best; three terms
-// (24 bits; six products, 2^-24 left out) for f32 weights.  One term where the factors are already
-// bf16, or both fp16.
+// has f32's range.  Two terms (16 bits of each factor; h h + h m + m h, what is left out is at most
+// 3 * 2^-16 of a product: the last bits of either factor, and m m) for weights of 8 or 16 bits, whose own rounding is 2^-11
+// of the result or more: it hides what is left out unless the products cancel to less than 3 * 2^-5 of their sizes' sum on a weight
+// near zero.  Three products instead of six; those of the [5120, 3456] cut with factors of rank 256 are what bounds that merge.
+// Three terms (24 bits; six products, what is left out is at most 4 * 2^-24) for f32 weights.  One term where the
+// factors are already bf16, or both fp16.
 //
 // Operand layout.  v_mfma_f32_16x16x32 takes 8 consecutive k of row lane % 16 from each lane
 // (k = 8 (lane / 16) + 0..7): a block of 16 rows x 32 k is stored as the 64 lanes' 16 bytes in

@@ -22,8 +22,9 @@ extern "C" {
 #endif
 
 /* dst = round(src + scale * (up @ down)); dst == src (same pitch) merges in place.
- * Products and sums are held in 32 bits; factors of f32 are split into bf16 terms, as many as the
- * weight's type can tell apart.  With FSTX_F8_E4M3 weights W stands for W * weight_scale[row] and the
+ * Products and sums are held in 32 bits; factors of f32 are split into bf16 terms, three for f32 weights
+ * (off by 4 * 2^-24 of each product at most) and two for others (3 * 2^-16, which their own rounding hides unless
+ * the products cancel).  With FSTX_F8_E4M3 weights W stands for W * weight_scale[row] and the
  * result is (W * weight_scale + scale * up @ down) / weight_scale, saturated to +-448 (a NaN stays one).
  * An infinity in a factor makes its row or column infinite or NaN.  Up to about
  * 6 * 10^9 elements, and 10^8 rows and columns together per 32 of the rank (-FSTX_E_RANGE). */
