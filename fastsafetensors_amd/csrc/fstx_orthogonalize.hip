@@ -143,7 +143,7 @@ __host__ __device__ inline uint32_t pad_to(uint32_t n, uint32_t to) { return (n 
 
 // N elements, those at(e) that are there(e), zeros else.  All loads go out together: the type is looked at once, and what
 // is not there is read from the matrix's first element and dropped (a branch around each load would wait for one after the other: the first operands
-// of a [14336, 4096] bf16 update 129 us instead of 186).
+// of a [14336, 4096] bf16 update 129 us instead of 186; 104 with the norm's sums added by plan_kernel).
 template <uint32_t N, typename At, typename There>
 __device__ __forceinline__ void load_elems(const char *src, uint32_t type, float (&x)[N], At at, There there) {
     if (type == FSTX_F32) {
@@ -345,7 +345,7 @@ template <uint32_t left> __device__ __forceinline__ void wait_and_meet() {
 template <uint32_t TR, uint32_t TC> struct Product {
     static constexpr uint32_t kKb = TR == 64 ? 2 : 1;                         // k blocks per stage
     // Stages in LDS: one computed on, the others on their way.  Small tiles run where few workgroups wait for
-    // each other's results from memory: four, [768, 768] fp32 155 us instead of 182, [1500, 3000] bf16 380 instead of 405 (five: the same).
+    // each other's results from memory: four, [768, 768] fp32 157 us instead of 176, [1024, 1024] bf16 187 instead of 204 (five: the same).
     static constexpr uint32_t kBufs = TR == 64 ? 4 : 3;
     static constexpr uint32_t kHalfP = TR / 32 * kKb * kTerms;                 // blocks of either operand per stage
     static constexpr uint32_t kHalfQ = TC / 32 * kKb * kTerms;
@@ -780,9 +780,10 @@ __global__ __launch_bounds__(64) void join_pieces_kernel(const Jobs t, const Dea
 // P A P loses that A is X X^T, whose eigenvalues are never negative: what rounding leaves of an eigenvalue of zero, +-2^-53,
 // grows by a^2 a step like that of any small direction, but a negative one without end (rank 1 and twenty steps of a = 3.4445: 1e40).
 // So steps are taken in runs in which a direction grows by kSlimGrowth at most, 2^26 times 2^-53 of an eigenvalue; between two runs
-// X = Q X is made, in 64 bits, and A taken from it anew.  The nine steps of a polar factor are one run.
+// X = Q X is made, in 64 bits, and A taken from it anew.  The nine steps of a polar factor are one run; fourteen steps of a = 15/8
+// too (a [32, 4096] fp32 update 45 us), fifteen are two (67 us), sixty-four five (197 us).
 //
-// A run is three launches and reads the update twice: with five steps a [1, 700] fp32 update takes 22 us instead of 101, [32, 4096] 31 instead of 119 and
+// A run is three launches and reads the update twice: with five steps a [1, 700] fp32 update takes 23 us instead of 101, [32, 4096] 32 instead of 119 and
 // [32, 28672] 50 instead of 287.  At 64 rows one workgroup's products would take as long as the launches they save.
 // The partial sums of M are added in a fixed order.
 
