@@ -26,7 +26,7 @@
 // fp16 rather than bf16 terms because the iterates are bounded: entries of X are at most about
 // 1.2, they are held times a power of two near sqrt(p q) so that their typical size stays in the
 // middle of fp16's range; A and B are held times powers of two likewise.  Where |G| is far below eps, or a step makes all singular values
-// small, these powers follow a bound of the singular values from step to step, for each matrix by itself: see Plan.
+// small, these powers follow a bound of the singular values from step to step, for each matrix by itself: see plan_kernel.
 //
 // Operand layout.  A matrix [R, K] that enters a product as rows x K is stored as blocks of 32
 // rows x 16 k in the lane order of v_mfma_f32_32x32x16 (lane: row lane % 32, k = 8 (lane / 32) + 0..7), 1 KiB
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256) void sum_squares_kernel(const Jobs t) {
 // at first, |a| s + |b| s^3 + |c| s^5 behind a step.  X is held times scale 2^e, s 2^e being just below 1 (e = 0 from s = 1/2 on), A times
 // kScaleA 2^(2 e), and B times the power of two up to which 4 |b| + 16 |c|, its largest entry for s = 2, stays below fp16's
 // largest, and for e > 0 another 2^g that puts the bound |b| s^2 + |c| s^4 there.  Held times fixed powers of two instead, an
-// update of |G| = 10^-7 eps lost all but six digits of its bits in fp16's denormals, and one of 10^-8 eps was zero.
+// update of |G| = 10^-6 eps came out 1.7 % off, with its digits in fp16's denormals, and one of 10^-8 eps as zero.
 // One wavefront per matrix; its partial sums are all read before the plan is written over them.
 __global__ __launch_bounds__(64) void plan_kernel(const Jobs t, const Steps steps) {
     const Job job = fetch_job(t, blockIdx.x);
